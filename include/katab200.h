@@ -178,6 +178,71 @@ int kb_conv_noalloc(
 /* Message of the last kb_conv_noalloc failure on the calling thread. */
 const char* kb_conv_noalloc_last_error(void);
 
+/* Transformer operators on the caller's own device buffers.  (No counterpart in the reference: there they exist inside a net
+ * only.)  Together they are a block whose tokens look at states of another length: project, rotate, attend, project again.
+ *
+ * Conventions of all of them:
+ *   - pointers are DEVICE addresses on the current device (managed memory is taken too); host memory and memory of another
+ *     device are refused.  Elements have the type that `precision` (KB_PRECISION_*) names, sums are held in fp32, a result is
+ *     rounded once;
+ *   - strides count elements and may be anything from 0 up for inputs (0 repeats); the innermost dimension is contiguous;
+ *     elements of an output must not coincide, and an output must not overlap an input unless the text below allows it;
+ *   - any alignment of the element type is taken; rows that start on 16-byte boundaries are fastest;
+ *   - the kernels are enqueued on `stream` (a cudaStream_t of the current device, NULL = its default stream) and the call
+ *     returns without waiting.  Calls may be captured into a graph, and made from several threads at once on different buffers;
+ *   - nothing is allocated and nothing kept from one call to the next (but a status word for the library, at the first call);
+ *   - non-zero and kb_last_error() as everywhere; a refused call has launched nothing.  A device-side wait that ran out (it never
+ *     does in sound operation) is reported by the next call of an operator.
+ * The same call on the same inputs gives the same bits. */
+
+/* Elements [batch][token][head][channel]; the channel is contiguous, the strides are in elements. */
+typedef struct kb_view {
+  void* data;
+  int64_t batchStride, tokenStride, headStride;
+} kb_view;
+
+/* y = act(x w^T + bias) + residual, the product of a projection or one half of a feed-forward layer.
+ *   x [m][k], rows ldx apart      w [n][k], rows ldw apart (the order of a tensor-core convolution's weights, outC x inC)
+ *   bias [n] fp32 or NULL         residual [m][n], rows ldr apart, or NULL
+ *   y [m][n], rows ldy apart      act a KB_ACT_* of kb_modelblob.h
+ * The residual may be y itself (same address, same stride).  m may be 0. */
+int kb_matmul(
+  int precision, int m, int n, int k, const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, int act,
+  const void* residual, int64_t ldr, void* y, int64_t ldy, void* stream);
+
+/* Rotary positions with any number of axes (time, row, column): pair p of a head is turned by
+ *   angle[b][t][p] = sum over a of positions[b][t][a] * freqs[table][p][a]     (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos)
+ *   positions [batch][tokens][axes] int32, sequences posBatchStride apart (0: all have the same); any value: the angle is reduced
+ *             to a fraction of a turn exactly, so far positions are as good as near ones
+ *   freqs     [freqHeads][rotDim/2][axes] fp32, radians per step; head h of H uses table h*freqHeads/H (freqHeads divides qHeads
+ *             and kHeads).  A pair that turns with one axis has zeros for the others
+ *   pairsInHalves 0: pair p is channels 2p, 2p+1 (as in the nets of this library); 1: channels p, p + rotDim/2
+ * The first rotDim of a head's headDim channels are turned, the others copied.  q and k are turned in one call; either may be
+ * absent (0 heads, views NULL).  An output may be its own input (same view: in place). */
+int kb_rope(
+  int precision, int batch, int tokens, int headDim, int rotDim, const int32_t* positions, int64_t posBatchStride, int axes,
+  const float* freqs, int freqHeads, int pairsInHalves, const kb_view* qIn, const kb_view* qOut, int qHeads, const kb_view* kIn,
+  const kb_view* kOut, int kHeads, void* stream);
+
+/* Attention of qLen tokens to the kLen states of another sequence (or of their own):
+ *   out[b][i][h] = sum over j of p[j] v[b][j][g],  p = softmax over j of scale * q[b][i][h] . k[b][j][g],  g = h*kvHeads/heads
+ *   q [batch][qLen][heads][qkDim]   k [batch][kLen][kvHeads][qkDim]   v [batch][kLen][kvHeads][vDim]
+ *   out [batch][qLen][heads][vDim]  head sizes 1..256, heads a multiple of kvHeads, scale > 0
+ *   qLengths, kLengths [batch] int32 on the device or NULL: rows of `out` from qLengths[b] on are left as they are; keys from
+ *             kLengths[b] on are not read.  Values outside 0..qLen / 0..kLen count as the nearer end
+ *   keyMask   [batch][kLen] fp32 or NULL: keys whose mask is 0 are left out, whatever their k and v hold (NaN and Inf included)
+ *   queryMask [batch][qLen] fp32 or NULL: tokens whose mask is 0 get a row of zeros
+ * A row that no key is left for is zeros.
+ *   workspace, workspaceBytes: device memory, 16-byte aligned, at least what kb_cross_attention_workspace says for the same sizes
+ *             (it depends on nothing else; 0 for most).  Its contents need not be set and mean nothing after the call; two
+ *             calls whose kernels overlap on the GPU (two streams, two graphs) need one each. */
+int kb_cross_attention_workspace(
+  int precision, int batch, int qLen, int kLen, int heads, int kvHeads, int qkDim, int vDim, size_t* bytes);
+int kb_cross_attention(
+  int precision, int batch, int qLen, int kLen, int heads, int kvHeads, int qkDim, int vDim, float scale, const kb_view* q,
+  const kb_view* k, const kb_view* v, const kb_view* out, const int32_t* qLengths, const int32_t* kLengths, const float* keyMask,
+  const float* queryMask, void* workspace, size_t workspaceBytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

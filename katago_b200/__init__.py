@@ -12,8 +12,13 @@ from .capi import (  # noqa: F401
     PRECISION_FP32,
     Handle,
     Model,
+    View,
     build_library,
+    cross_attention,
+    cross_attention_workspace,
     device_count,
     eval_layer,
     library_path,
+    matmul,
+    rope,
 )

@@ -20,12 +20,18 @@ EXPORTED_SYMBOLS = [
     "kb_upload_inputs", "kb_forward_resident", "kb_download_outputs", "kb_time_forward_resident", "kb_time_forward_steps",
     "kb_profile_enable", "kb_profile_reset", "kb_profile_read", "kb_launches_per_forward", "kb_debug_read_trunk",
     "kb_eval_layer", "kb_host_alloc", "kb_host_free", "kb_conv_noalloc", "kb_conv_noalloc_last_error",
+    "kb_matmul", "kb_rope", "kb_cross_attention_workspace", "kb_cross_attention",
 ]
 
 
 class ProfileEntry(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 48), ("launches", ctypes.c_int64), ("ms", ctypes.c_double),
                 ("flops", ctypes.c_double), ("bytes", ctypes.c_double)]
+
+
+class View(ctypes.Structure):
+    """kb_view: elements [batch][token][head][channel] at a device address; strides in elements, channels contiguous."""
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
 
 
 def library_path() -> str:
@@ -80,6 +86,11 @@ def lib():
         L.kb_host_free.argtypes = [vp]
         L.kb_conv_noalloc.argtypes = [vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, vp]
         L.kb_conv_noalloc_last_error.restype = ctypes.c_char_p
+        i64, view = ctypes.c_int64, ctypes.POINTER(View)
+        L.kb_matmul.argtypes = [ci] * 4 + [vp, i64, vp, i64, vp, ci, vp, i64, vp, i64, vp]
+        L.kb_rope.argtypes = [ci] * 5 + [vp, i64, ci, vp, ci, ci, view, view, ci, view, view, ci, vp]
+        L.kb_cross_attention_workspace.argtypes = [ci] * 8 + [ctypes.POINTER(sz)]
+        L.kb_cross_attention.argtypes = [ci] * 8 + [ctypes.c_float, view, view, view, view, vp, vp, vp, vp, vp, sz, vp]
         _lib = L
     return _lib
 
@@ -277,6 +288,39 @@ def conv_noalloc(d_in: int, d_weights: int, d_out: int, n: int, nn_x: int, nn_y:
     status = lib().kb_conv_noalloc(d_in, d_weights, d_out, n, nn_x, nn_y, in_c, out_c, ky, kx, stream or None)
     if status != 0:
         raise KBError(f"kb_conv_noalloc failed ({status}): {lib().kb_conv_noalloc_last_error().decode()}")
+
+
+def matmul(precision: int, m: int, n: int, k: int, x: int, ldx: int, w: int, ldw: int, y: int, ldy: int, bias: int = 0, act: int = 0,
+           residual: int = 0, ldr: int = 0, stream: int = 0) -> None:
+    """kb_matmul with raw device addresses (ints): y = act(x w^T + bias) + residual.  Enqueues on `stream`."""
+    if lib().kb_matmul(precision, m, n, k, x, ldx, w, ldw, bias, act, residual, ldr, y, ldy, stream):
+        _check(1, "kb_matmul")
+
+
+def rope(precision: int, batch: int, tokens: int, head_dim: int, rot_dim: int, positions: int, pos_batch_stride: int, axes: int, freqs: int,
+         freq_heads: int, pairs_in_halves: int, q_in: View, q_out: View, q_heads: int, k_in: View = None, k_out: View = None, k_heads: int = 0,
+         stream: int = 0) -> None:
+    """kb_rope: turns the pairs of q's and k's heads by positions with several axes.  Enqueues on `stream`."""
+    if lib().kb_rope(precision, batch, tokens, head_dim, rot_dim, positions, pos_batch_stride, axes, freqs, freq_heads, pairs_in_halves,
+                     q_in, q_out, q_heads, k_in, k_out, k_heads, stream):
+        _check(1, "kb_rope")
+
+
+def cross_attention_workspace(precision: int, batch: int, q_len: int, k_len: int, heads: int, kv_heads: int, qk_dim: int, v_dim: int) -> int:
+    """Bytes of device memory that kb_cross_attention needs for these sizes."""
+    n = ctypes.c_size_t()
+    _check(lib().kb_cross_attention_workspace(precision, batch, q_len, k_len, heads, kv_heads, qk_dim, v_dim, ctypes.byref(n)),
+           "kb_cross_attention_workspace")
+    return n.value
+
+
+def cross_attention(precision: int, batch: int, q_len: int, k_len: int, heads: int, kv_heads: int, qk_dim: int, v_dim: int, scale: float,
+                    q: View, k: View, v: View, out: View, q_lengths: int = 0, k_lengths: int = 0, key_mask: int = 0, query_mask: int = 0,
+                    workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
+    """kb_cross_attention: attention of q_len tokens to k_len states.  Enqueues on `stream`."""
+    if lib().kb_cross_attention(precision, batch, q_len, k_len, heads, kv_heads, qk_dim, v_dim, scale, q, k, v, out, q_lengths, k_lengths,
+                                key_mask, query_mask, workspace, workspace_bytes, stream):
+        _check(1, "kb_cross_attention")
 
 
 def eval_layer(blob: bytes, x: np.ndarray, mask, out_c: int, precision: int = PRECISION_FP32, device: int = -1) -> np.ndarray:

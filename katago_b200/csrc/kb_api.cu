@@ -7,6 +7,7 @@
 #include <string>
 
 #include "kb_engine.h"
+#include "kb_ops.h"
 #include "kb_tile_table.h"
 
 struct kb_model {
@@ -219,6 +220,48 @@ int kb_eval_layer(
   return guarded([&]() {
     kb::Engine e(blob, nbytes, device, n, nnXLen, nnYLen, precision);
     e.evalLayer(in, mask, out);
+  });
+}
+
+int kb_matmul(
+  int precision, int m, int n, int k, const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, int act,
+  const void* residual, int64_t ldr, void* y, int64_t ldy, void* stream) {
+  return guarded([&]() {
+    kb::MatmulArgs a = {};
+    a.dt = precision; a.M = m; a.N = n; a.K = k;
+    a.x = x; a.ldx = ldx; a.w = w; a.ldw = ldw; a.bias = bias; a.act = act;
+    a.residual = residual; a.ldr = ldr; a.y = y; a.ldy = ldy;
+    kb::opMatmul(a, stream);
+  });
+}
+int kb_rope(
+  int precision, int batch, int tokens, int headDim, int rotDim, const int32_t* positions, int64_t posBatchStride, int axes,
+  const float* freqs, int freqHeads, int pairsInHalves, const kb_view* qIn, const kb_view* qOut, int qHeads, const kb_view* kIn,
+  const kb_view* kOut, int kHeads, void* stream) {
+  return guarded([&]() {
+    kb::RopeArgs a = {};
+    a.dt = precision; a.batch = batch; a.tokens = tokens; a.dim = headDim; a.rot = rotDim;
+    a.positions = positions; a.posB = posBatchStride; a.axes = axes; a.freqs = freqs; a.freqHeads = freqHeads; a.halves = pairsInHalves;
+    a.q.heads = qHeads; a.k.heads = kHeads;
+    kb::opRope(a, qIn, qOut, kIn, kOut, stream);
+  });
+}
+int kb_cross_attention_workspace(
+  int precision, int batch, int qLen, int kLen, int heads, int kvHeads, int qkDim, int vDim, size_t* bytes) {
+  return guarded([&]() {
+    need(bytes, "bytes");
+    *bytes = kb::opCrossAttnWorkspace(precision, batch, qLen, kLen, heads, kvHeads, qkDim, vDim);
+  });
+}
+int kb_cross_attention(
+  int precision, int batch, int qLen, int kLen, int heads, int kvHeads, int qkDim, int vDim, float scale, const kb_view* q,
+  const kb_view* k, const kb_view* v, const kb_view* out, const int32_t* qLengths, const int32_t* kLengths, const float* keyMask,
+  const float* queryMask, void* workspace, size_t workspaceBytes, void* stream) {
+  return guarded([&]() {
+    kb::CrossAttnArgs a = {};
+    a.dt = precision; a.batch = batch; a.qLen = qLen; a.kLen = kLen; a.heads = heads; a.kvHeads = kvHeads; a.dq = qkDim; a.dv = vDim;
+    a.scale = scale; a.qLengths = qLengths; a.kLengths = kLengths; a.keyMask = keyMask; a.queryMask = queryMask; a.workspace = workspace;
+    kb::opCrossAttn(a, q, k, v, out, workspaceBytes, stream);
   });
 }
 

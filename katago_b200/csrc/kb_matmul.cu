@@ -1,0 +1,201 @@
+// y = act(x w^T + bias) + residual on a caller's own matrices, on the CUDA cores: fp32, and 16-bit matrices whose rows do not
+// start on the boundaries that TMA needs.  (16-bit matrices with aligned rows: kb_matmul_tc.cu.)
+//
+// matmulTileKernel   one tile of BM x BN outputs per block, 16 elements of K staged at a time in fp32, double-buffered: the
+//                    next slice travels through registers while this one is multiplied.  FMA-bound; pairs of neighbouring
+//                    outputs use the packed fp32 instructions (two IEEE operations per issue slot).
+// matmulFewKernel    up to eight rows: memory-bound, the weights are read once.  A block has four weight rows and cuts K
+//                    over its warps, whose sums are added in warp order.
+#include "kb_kernels.cuh"
+#include "kb_ops.h"
+#include "kb_ops_dev.cuh"
+
+#include <algorithm>
+
+namespace kb {
+
+namespace {
+
+template <typename T>
+__device__ __forceinline__ void matmulStore(const MatmulArgs& a, int m, int n, float v) {
+  if(a.bias) v += a.bias[n];
+  v = opAct<T>(v, a.act);
+  if(a.residual) v += OpType<T>::to(((const T*)a.residual)[(int64_t)m * a.ldr + n]);
+  ((T*)a.y)[(int64_t)m * a.ldy + n] = OpType<T>::from(v);
+}
+
+// V: elements of K per global access
+template <typename T, int BM, int BN, int V>
+__global__ void __launch_bounds__(256) matmulTileKernel(const MatmulArgs a) {
+  constexpr int BK = 16, TM = BM / 16, TN = BN / 16;
+  constexpr int PA = BM + 4, PB = BN + 4;  // pitches: rows of 16 bytes, transposed stores spread over the banks
+  __shared__ __align__(16) float sA[2][BK][PA], sB[2][BK][PB];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int tilesN = (a.N + BN - 1) / BN;
+  const long long tile = blockIdx.x;
+  const int m0 = (int)(tile / tilesN) * BM, n0 = (int)(tile % tilesN) * BN;
+  constexpr int PER_ROW = BK / V;                  // accesses per staged row
+  constexpr int ROWS = 256 / PER_ROW;              // rows per pass
+  constexpr int NA = (BM + ROWS - 1) / ROWS, NB = (BN + ROWS - 1) / ROWS;
+  const int lk = (tid % PER_ROW) * V, lr = tid / PER_ROW;
+  OpVec<T, V> ra[NA], rb[NB];
+  gridDepLaunch();
+  gridDepWait();
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for(int i = 0; i < NA; i++) {
+      const int r = lr + i * ROWS, m = m0 + r, k = k0 + lk;
+#pragma unroll
+      for(int e = 0; e < V; e++) ra[i].e[e] = OpType<T>::from(0.0f);
+      if(r < BM && m < a.M && k < a.K) ra[i].load((const T*)a.x + (int64_t)m * a.ldx + k);  // K is a multiple of V
+    }
+#pragma unroll
+    for(int i = 0; i < NB; i++) {
+      const int r = lr + i * ROWS, n = n0 + r, k = k0 + lk;
+#pragma unroll
+      for(int e = 0; e < V; e++) rb[i].e[e] = OpType<T>::from(0.0f);
+      if(r < BN && n < a.N && k < a.K) rb[i].load((const T*)a.w + (int64_t)n * a.ldw + k);
+    }
+  };
+  auto stage = [&](int s) {
+#pragma unroll
+    for(int i = 0; i < NA; i++)
+      if(lr + i * ROWS < BM)
+#pragma unroll
+        for(int e = 0; e < V; e++) sA[s][lk + e][lr + i * ROWS] = OpType<T>::to(ra[i].e[e]);
+#pragma unroll
+    for(int i = 0; i < NB; i++)
+      if(lr + i * ROWS < BN)
+#pragma unroll
+        for(int e = 0; e < V; e++) sB[s][lk + e][lr + i * ROWS] = OpType<T>::to(rb[i].e[e]);
+  };
+  // thread (ty, tx): rows ty*4.. of every 64, columns tx*4.. of every 64 (TM and TN are multiples of 4, or the tile is 32 wide: 2)
+  constexpr int CM = TM >= 4 ? 4 : TM, CN = TN >= 4 ? 4 : TN;
+  float2 acc[TM][TN / 2];
+#pragma unroll
+  for(int i = 0; i < TM; i++)
+#pragma unroll
+    for(int j = 0; j < TN / 2; j++) acc[i][j] = make_float2(0.0f, 0.0f);
+  const int steps = (a.K + BK - 1) / BK;
+  fetch(0);
+  stage(0);
+  __syncthreads();
+  for(int s = 0; s < steps; s++) {
+    if(s + 1 < steps) fetch((s + 1) * BK);
+    const int cur = s & 1;
+#pragma unroll
+    for(int k = 0; k < BK; k++) {
+      float av[TM];
+      float2 bv[TN / 2];
+#pragma unroll
+      for(int i = 0; i < TM / CM; i++)
+#pragma unroll
+        for(int e = 0; e < CM; e++) av[i * CM + e] = sA[cur][k][i * 16 * CM + ty * CM + e];
+#pragma unroll
+      for(int j = 0; j < TN / CN; j++)
+#pragma unroll
+        for(int e = 0; e < CN / 2; e++) bv[j * (CN / 2) + e] = *reinterpret_cast<const float2*>(&sB[cur][k][j * 16 * CN + tx * CN + 2 * e]);
+#pragma unroll
+      for(int i = 0; i < TM; i++)
+#pragma unroll
+        for(int j = 0; j < TN / 2; j++) acc[i][j] = __ffma2_rn(make_float2(av[i], av[i]), bv[j], acc[i][j]);
+    }
+    if(s + 1 < steps) stage(cur ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for(int i = 0; i < TM; i++) {
+    const int m = m0 + (i / CM) * 16 * CM + ty * CM + i % CM;
+    if(m >= a.M) continue;
+#pragma unroll
+    for(int j = 0; j < TN; j++) {
+      const int n = n0 + (j / CN) * 16 * CN + tx * CN + j % CN;
+      if(n < a.N) matmulStore<T>(a, m, n, j % 2 == 0 ? acc[i][j / 2].x : acc[i][j / 2].y);
+    }
+  }
+}
+
+constexpr int FEW_COLS = 4;
+
+// MR rows (1, 2, 4 or 8; rows past M repeat the last one and are not stored)
+template <typename T, int MR, int V>
+__global__ void __launch_bounds__(256) matmulFewKernel(const MatmulArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * FEW_COLS;
+  float acc[MR][FEW_COLS];
+#pragma unroll
+  for(int m = 0; m < MR; m++)
+#pragma unroll
+    for(int c = 0; c < FEW_COLS; c++) acc[m][c] = 0.0f;
+  gridDepLaunch();
+  gridDepWait();
+  for(int k = (warp * 32 + lane) * V; k < a.K; k += 8 * 32 * V) {
+    OpVec<T, V> w[FEW_COLS];
+#pragma unroll
+    for(int c = 0; c < FEW_COLS; c++) w[c].load((const T*)a.w + (int64_t)min(n0 + c, a.N - 1) * a.ldw + k);
+#pragma unroll
+    for(int m = 0; m < MR; m++) {
+      OpVec<T, V> x;
+      x.load((const T*)a.x + (int64_t)min(m, a.M - 1) * a.ldx + k);
+#pragma unroll
+      for(int e = 0; e < V; e++) {
+        const float xe = OpType<T>::to(x.e[e]);
+#pragma unroll
+        for(int c = 0; c < FEW_COLS; c++) acc[m][c] = fmaf(xe, OpType<T>::to(w[c].e[e]), acc[m][c]);
+      }
+    }
+  }
+  __shared__ float part[8][MR * FEW_COLS];
+#pragma unroll
+  for(int m = 0; m < MR; m++)
+#pragma unroll
+    for(int c = 0; c < FEW_COLS; c++) {
+      float v = acc[m][c];
+#pragma unroll
+      for(int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+      if(lane == 0) part[warp][m * FEW_COLS + c] = v;
+    }
+  __syncthreads();
+  for(int i = threadIdx.x; i < MR * FEW_COLS; i += 256) {
+    const int m = i / FEW_COLS, n = n0 + i % FEW_COLS;
+    if(m >= a.M || n >= a.N) continue;
+    float v = 0.0f;
+#pragma unroll
+    for(int s = 0; s < 8; s++) v += part[s][i];
+    matmulStore<T>(a, m, n, v);
+  }
+}
+
+template <typename T, int V> cudaError_t matmulLaunch(cudaStream_t st, const MatmulArgs& a) {
+  if(a.M <= 8) {
+    const dim3 grid((a.N + FEW_COLS - 1) / FEW_COLS), block(256);
+    if(a.M == 1) return launchDependent(matmulFewKernel<T, 1, V>, grid, block, 0, st, a);
+    if(a.M == 2) return launchDependent(matmulFewKernel<T, 2, V>, grid, block, 0, st, a);
+    if(a.M <= 4) return launchDependent(matmulFewKernel<T, 4, V>, grid, block, 0, st, a);
+    return launchDependent(matmulFewKernel<T, 8, V>, grid, block, 0, st, a);
+  }
+  constexpr int VT = V > 4 ? 4 : V;  // elements of the tile kernel's accesses: four threads per staged row
+  auto tiles = [&](int bm, int bn) { return ((long long)a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
+  const int sms = smCount();
+  if(tiles(128, 128) >= 2 * sms) return launchDependent(matmulTileKernel<T, 128, 128, VT>, dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, a);
+  if(tiles(64, 64) >= sms) return launchDependent(matmulTileKernel<T, 64, 64, VT>, dim3((unsigned)tiles(64, 64)), dim3(256), 0, st, a);
+  return launchDependent(matmulTileKernel<T, 32, 32, VT>, dim3((unsigned)tiles(32, 32)), dim3(256), 0, st, a);
+}
+
+template <typename T> cudaError_t matmulLaunchT(cudaStream_t st, const MatmulArgs& a) {
+  constexpr int V = 16 / sizeof(T);
+  const bool vec = (((uintptr_t)a.x | (uintptr_t)a.w) & 15) == 0 && (a.ldx % V) == 0 && (a.ldw % V) == 0 && a.K % V == 0;
+  return vec ? matmulLaunch<T, V>(st, a) : matmulLaunch<T, 1>(st, a);
+}
+
+}  // namespace
+
+cudaError_t launchMatmul(cudaStream_t st, const MatmulArgs& a) {
+  switch(a.dt) {
+    case DT_F32: return matmulLaunchT<float>(st, a);
+    case DT_F16: return matmulLaunchT<__half>(st, a);
+    default: return matmulLaunchT<__nv_bfloat16>(st, a);
+  }
+}
+
+}  // namespace kb

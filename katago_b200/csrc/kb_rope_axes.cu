@@ -1,0 +1,168 @@
+// Rotary positions with several axes on a caller's own tensors.
+//
+//   angle(t, p) = sum_a position[t][a] * freq[p][a]
+//   (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos)      for every pair p of every head
+//
+// What bounds it: memory.  Every channel is read and written once; cosine and sine are computed once per token and pair and
+// used for all heads that one thread walks through.
+//
+// Angles of far positions.  position * freq in fp32 is off by 2^-24 of the ANGLE: half a turn at a position of a few million.
+// Only the angle's fraction of a turn matters, and that is arithmetic modulo one: a frequency is turned into turns per step as
+// a 64-bit fixed-point fraction (computed in fp64 with the rest of 1/2pi behind its leading word), the product with an integer
+// position wraps by itself, and the sum over the axes does too.  What is left is a signed fraction of a turn, of which the upper
+// 32 bits go to sincospif: 2^-32 of a turn, at any int32 position (the frequency's own fraction is good to 2^-64, times a
+// position of 2^31 at worst 2^-33).
+#include "kb_kernels.cuh"
+#include "kb_ops.h"
+#include "kb_ops_dev.cuh"
+
+#include <algorithm>
+
+namespace kb {
+
+namespace {
+
+// 1 / (2 pi) in two doubles.
+constexpr double INV_2PI_HI = 0.15915494309189535;
+constexpr double INV_2PI_LO = -9.839338337591243e-18;
+
+// Turns per step of one position as a fraction of 2^64.
+__device__ __forceinline__ unsigned long long turnFraction(float freq) {
+  const double f = (double)freq;
+  const double hi = f * INV_2PI_HI;
+  const double lo = fma(f, INV_2PI_HI, -hi) + f * INV_2PI_LO;
+  const double frac = (hi - rint(hi)) + lo;  // [-0.5, 0.5] and a little
+  // scaled by 2^63 (no overflow at +-0.5) and doubled in the ring
+  return 2ull * (unsigned long long)__double2ll_rn(frac * 9223372036854775808.0);
+}
+
+// MODE 0: scalar pairs (any alignment), 1: V elements = V/2 adjacent pairs per access, 2: halves, V pairs per two accesses
+template <typename T, int MODE, int V>
+__global__ void __launch_bounds__(256) ropeAxesKernel(const RopeArgs a, int chunks, int rotChunks, int headsPerItem, int headGroups, long long items) {
+  gridDepLaunch();
+  gridDepWait();
+  constexpr int P = MODE == 0 ? 1 : (MODE == 1 ? V / 2 : V);
+  const int pairs = a.rot / 2;
+  const int totalHeads = a.q.heads + a.k.heads;
+  for(long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x; item < items; item += (long long)gridDim.x * blockDim.x) {
+    // chunk fastest, then token, then group of heads: neighbouring threads touch neighbouring memory
+    const long long rest = item / chunks;
+    const int c = (int)(item - rest * chunks);
+    const long long tokensAll = (long long)a.batch * a.tokens;
+    const int hg = (int)(rest / tokensAll);
+    const long long bt = rest - hg * tokensAll;
+    const int b = (int)(bt / a.tokens), t = (int)(bt - (long long)b * a.tokens);
+    const int h0 = hg * headsPerItem, h1 = min(totalHeads, h0 + headsPerItem);
+    const T* qIn = (const T*)a.q.in + b * a.q.inB + t * a.q.inT;
+    const T* kIn = (const T*)a.k.in + b * a.k.inB + t * a.k.inT;
+    T* qOut = (T*)a.q.out + b * a.q.outB + t * a.q.outT;
+    T* kOut = (T*)a.k.out + b * a.k.outB + t * a.k.outT;
+    auto in = [&](int h) { return h < a.q.heads ? qIn + h * a.q.inH : kIn + (h - a.q.heads) * a.k.inH; };
+    auto out = [&](int h) { return h < a.q.heads ? qOut + h * a.q.outH : kOut + (h - a.q.heads) * a.k.outH; };
+    if(c >= rotChunks) {  // channels without a position
+      constexpr int W = MODE == 0 ? 1 : V;
+      const int e = a.rot + (c - rotChunks) * W;
+      for(int h = h0; h < h1; h++) {
+        OpVec<T, W> v;
+        v.load(in(h) + e);
+        v.store(out(h) + e);
+      }
+      continue;
+    }
+    float cs[P], sn[P];
+    int table = -1;
+    const int32_t* pos = a.positions + b * a.posB + (long long)t * a.axes;
+    auto angles = [&](int th) {
+      table = th;
+      const float* f = a.freqs + ((size_t)th * pairs + (size_t)c * P) * a.axes;
+#pragma unroll
+      for(int p = 0; p < P; p++) {
+        unsigned long long turn = 0;
+        bool finite = true;
+        for(int x = 0; x < a.axes; x++) {
+          const float fr = f[p * a.axes + x];
+          finite = finite && isfinite(fr);
+          turn += turnFraction(fr) * (unsigned long long)(long long)pos[x];
+        }
+        // upper 32 bits as a signed fraction: units of half a turn for sincospif
+        const float halfTurns = finite ? (float)(int)(turn >> 32) * 4.656612873077393e-10f : __int_as_float(0x7fffffff);
+        sincospif(halfTurns, &sn[p], &cs[p]);
+      }
+    };
+    auto tableOf = [&](int h) {
+      return a.freqHeads == 1 ? 0 : (h < a.q.heads ? h / (a.q.heads / a.freqHeads) : (h - a.q.heads) / (a.k.heads / a.freqHeads));
+    };
+    constexpr int U = 4;  // heads whose loads are in flight together
+    for(int hb = h0; hb < h1; hb += U) {
+      constexpr int NV = MODE == 1 ? 1 : 2;
+      constexpr int W = MODE == 0 ? 1 : V;
+      OpVec<T, W> v[U][NV];
+      // the two places of a scalar pair, or the vector(s)
+      const int e0 = MODE == 0 ? (a.halves ? c : 2 * c) : c * V;
+      const int e1 = MODE == 0 ? (a.halves ? c + pairs : 2 * c + 1) : c * V + pairs;
+#pragma unroll
+      for(int u = 0; u < U; u++)
+        if(hb + u < h1) {
+          v[u][0].load(in(hb + u) + e0);
+          if(NV == 2) v[u][NV - 1].load(in(hb + u) + e1);
+        }
+#pragma unroll
+      for(int u = 0; u < U; u++) {
+        if(hb + u >= h1) break;
+        const int th = tableOf(hb + u);
+        if(th != table) angles(th);
+#pragma unroll
+        for(int p = 0; p < P; p++) {
+          T& r0 = MODE == 1 ? v[u][0].e[(2 * p) % W] : v[u][0].e[p % W];
+          T& r1 = MODE == 1 ? v[u][0].e[(2 * p + 1) % W] : v[u][NV - 1].e[p % W];
+          const float x0 = OpType<T>::to(r0), x1 = OpType<T>::to(r1);
+          r0 = OpType<T>::from(x0 * cs[p] - x1 * sn[p]);
+          r1 = OpType<T>::from(x0 * sn[p] + x1 * cs[p]);
+        }
+        v[u][0].store(out(hb + u) + e0);
+        if(NV == 2) v[u][NV - 1].store(out(hb + u) + e1);
+      }
+    }
+  }
+}
+
+template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a) {
+  constexpr int V = 16 / sizeof(T);
+  auto aligned = [&](const RopeHeads& h) {
+    if(h.heads == 0) return true;
+    const uintptr_t p = (uintptr_t)h.in | (uintptr_t)h.out;
+    const int64_t s = h.inB | h.inT | h.inH | h.outB | h.outT | h.outH;
+    return (p & 15) == 0 && (s % V) == 0;
+  };
+  const int unit = a.halves ? 2 * V : V;  // elements that one thread rotates
+  const bool vec = aligned(a.q) && aligned(a.k) && a.rot % unit == 0 && a.dim % V == 0;
+  // in place the channels behind the rotated ones stay as they are
+  const bool copy = (a.q.heads && a.q.in != a.q.out) || (a.k.heads && a.k.in != a.k.out);
+  const int rotChunks = vec ? a.rot / unit : a.rot / 2;
+  const int chunks = rotChunks + (copy ? (vec ? (a.dim - a.rot) / V : a.dim - a.rot) : 0);
+  const int heads = a.q.heads + a.k.heads;
+  const long long perHead = (long long)a.batch * a.tokens * chunks;
+  if(perHead == 0 || heads == 0) return cudaSuccess;
+  // heads that one thread walks through: all of them (one set of angles), unless the threads would not fill the GPU
+  const long long want = 2048LL * smCount();
+  const int groups = (int)std::min<long long>(heads, std::max<long long>(1, want / perHead));
+  const int headsPerItem = (heads + groups - 1) / groups, headGroups = (heads + headsPerItem - 1) / headsPerItem;
+  const long long items = perHead * headGroups;
+  const long long blocks = std::min<long long>((items + 255) / 256, 1LL << 30);
+  const dim3 grid((unsigned)blocks), block(256);
+  if(!vec) return launchDependent(ropeAxesKernel<T, 0, 1>, grid, block, 0, st, a, chunks, rotChunks, headsPerItem, headGroups, items);
+  if(a.halves) return launchDependent(ropeAxesKernel<T, 2, V>, grid, block, 0, st, a, chunks, rotChunks, headsPerItem, headGroups, items);
+  return launchDependent(ropeAxesKernel<T, 1, V>, grid, block, 0, st, a, chunks, rotChunks, headsPerItem, headGroups, items);
+}
+
+}  // namespace
+
+cudaError_t launchRopeAxes(cudaStream_t st, const RopeArgs& a) {
+  switch(a.dt) {
+    case DT_F32: return ropeLaunch<float>(st, a);
+    case DT_F16: return ropeLaunch<__half>(st, a);
+    default: return ropeLaunch<__nv_bfloat16>(st, a);
+  }
+}
+
+}  // namespace kb
