@@ -191,6 +191,7 @@ template <typename T> cudaError_t matmulLaunchT(cudaStream_t st, const MatmulArg
 }  // namespace
 
 cudaError_t launchMatmul(cudaStream_t st, const MatmulArgs& a) {
+  if(a.M > 8 && matmulTcEligible(a)) return launchMatmulTc(st, a);
   switch(a.dt) {
     case DT_F32: return matmulLaunchT<float>(st, a);
     case DT_F16: return matmulLaunchT<__half>(st, a);

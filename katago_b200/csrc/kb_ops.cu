@@ -152,6 +152,37 @@ void checkLaunch(const char* op, cudaError_t e) {
 
 }  // namespace
 
+cudaError_t SharedMemoryOptIn::operator()(const void* fn, int bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if(e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+  if(done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = allowSharedMemory(fn, bytes);
+  if(e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+  return e;
+}
+
+bool encodeTiled(
+  CUtensorMap* map, int dt, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+  typedef CUresult (*EncodeFn)(
+    CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+    CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const EncodeFn fn = []() -> EncodeFn {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+    return reinterpret_cast<EncodeFn>(p);
+  }();
+  if(!fn) return false;
+  const CUtensorMapDataType type = dt == DT_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : (dt == DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+  cuuint64_t d[4], s[3];
+  cuuint32_t b[4], one[4] = {1, 1, 1, 1};
+  for(int i = 0; i < rank; i++) { d[i] = dims[i]; b[i] = box[i]; if(i > 0) s[i - 1] = strides[i - 1]; }
+  return fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 void opMatmul(const MatmulArgs& given, void* stream) {
   const char* op = "kb_matmul";
   MatmulArgs a = given;

@@ -2,13 +2,24 @@
 // kb_cross_attention): argument records, what kb_ops.cu checks, and the launchers of the kernels.
 #pragma once
 
+#include <cuda.h>
 #include <cuda_runtime.h>
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
 #include "../../include/katab200.h"
 
 namespace kb {
+
+// Lets `fn` use up to `bytes` of shared memory on the current device; asked of the driver once per device.
+struct SharedMemoryOptIn {
+  std::atomic<uint64_t> done{0};
+  cudaError_t operator()(const void* fn, int bytes);
+};
+// A tensor map of up to four dimensions (strides in bytes, of dimensions 1..); false if the driver refuses it.
+bool encodeTiled(
+  CUtensorMap* map, int dt, const void* base, int rank, const uint64_t* dims, const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle);
 
 // ---- y = act(x w^T + bias) + residual ----
 struct MatmulArgs {
@@ -23,6 +34,9 @@ struct MatmulArgs {
   int* status;                 // receives the code of a device-side wait that ran out
 };
 cudaError_t launchMatmul(cudaStream_t st, const MatmulArgs& a);
+// kb_matmul_tc.cu: 16-bit types, rows of x and w on 16-byte boundaries
+bool matmulTcEligible(const MatmulArgs& a);
+cudaError_t launchMatmulTc(cudaStream_t st, const MatmulArgs& a);
 
 // ---- rotary positions ----
 struct RopeHeads {

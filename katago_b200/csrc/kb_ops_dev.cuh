@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "kb_act.cuh"
 #include "kb_tc_ptx.cuh"
@@ -42,5 +43,44 @@ template <typename T, int V> struct OpVec {
 // Activations: exact functions for fp32 results, the special-function forms of the convolutions' epilogues for 16-bit ones
 // (their error is far below the rounding of the result).
 template <typename T> __device__ __forceinline__ float opAct(float v, int act) { return sizeof(T) == 4 ? applyActF(v, act) : fastAct(v, act); }
+
+// Bounded wait of a role of these kernels (about 2 s).  A wait that runs out raises the abort flag and leaves `code` in the status
+// word, which is page-locked host memory (hence a plain store); it returns false, as does one that finds the flag raised, and
+// the role then leaves its loops.
+static __device__ __noinline__ bool opWaitOn(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
+  const uint64_t t0 = globalTimerNs();
+  for(uint32_t spins = 1;; spins++) {
+    if(mbarTryWait(bar, parity)) return true;
+    if((spins & 63u) == 0u) {
+      if(*abortFlag) return false;
+      if(globalTimerNs() - t0 > 2000000000ull) {
+        *abortFlag = 1;
+        *status = code;
+        __threadfence_system();
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool opWait(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
+  return mbarTryWait(bar, parity) != 0u || opWaitOn(bar, parity, abortFlag, status, code);
+}
+
+// Two values in one 32-bit word of the 16-bit type, the first in the low half.
+template <typename T> __device__ __forceinline__ uint32_t opPack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t opPack<__half>(float lo, float hi) { const __half2 h = __floats2half2_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&h); }
+template <> __device__ __forceinline__ uint32_t opPack<__nv_bfloat16>(float lo, float hi) { const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&h); }
+template <typename T> __device__ __forceinline__ float2 opUnpack(uint32_t u);
+template <> __device__ __forceinline__ float2 opUnpack<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+template <> __device__ __forceinline__ float2 opUnpack<__nv_bfloat16>(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
+
+// Instruction descriptor of tcgen05.mma kind::f16 with fp32 accumulators: both operands of type T, K-major (bMn: B is MN-major).
+template <typename T> __host__ __device__ constexpr uint32_t opIdesc(int m, int n, bool bMn = false) {
+  const uint32_t fmt = sizeof(T) == 2 && !std::is_same<T, __half>::value ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (bMn ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// Words of a shared-memory matrix descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart (kb_tc_ptx.cuh, makeSmemDesc).
+constexpr uint32_t OP_DESC_HI = (uint32_t)(1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t opDescLo(uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | (1u << 16); }
 
 }  // namespace kb
