@@ -66,6 +66,33 @@ __device__ __forceinline__ bool opWait(uint32_t bar, uint32_t parity, volatile i
   return mbarTryWait(bar, parity) != 0u || opWaitOn(bar, parity, abortFlag, status, code);
 }
 
+__device__ __forceinline__ void tmaLoad4d(uint32_t dst, const CUtensorMap* tmap, int c0, int c1, int c2, int c3, uint32_t bar) {
+  asm volatile(
+    "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+    ::"r"(dst), "l"(tmap), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+    : "memory");
+}
+
+// 32 lanes x 16 consecutive columns -> 16 registers per thread, and the wait that names them (kb_tc_ptx.cuh, tmemLd32).
+__device__ __forceinline__ void tmemLd16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void tmemLdWaitFor(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
+}
+
+// The same in line, for kernels that move registers between warpgroups (ptxas finds no allocation with a call in them).
+__device__ __forceinline__ bool opWaitInline(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
+  if(mbarWait(bar, parity, abortFlag)) return true;
+  if(*abortFlag == 0) {
+    *abortFlag = 1;
+    *status = code;
+    __threadfence_system();
+  }
+  return false;
+}
+
 // Two values in one 32-bit word of the 16-bit type, the first in the low half.
 template <typename T> __device__ __forceinline__ uint32_t opPack(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t opPack<__half>(float lo, float hi) { const __half2 h = __floats2half2_rn(lo, hi); return *reinterpret_cast<const uint32_t*>(&h); }

@@ -230,7 +230,9 @@ template <typename T> cudaError_t simtLaunchT(cudaStream_t st, const CrossAttnAr
   return simtLaunch<T, 4>(st, a, sp);
 }
 
-XaSplit planSplit(int rowsPerBlock, int keysPerStep, int blocksPerSm, int batch, int qLen, int kLen, int heads, int kvHeads, int dv) {
+}  // namespace
+
+XaSplit xaPlanSplit(int rowsPerBlock, int keysPerStep, int blocksPerSm, int batch, int qLen, int kLen, int heads, int kvHeads, int dv) {
   XaSplit sp;
   const long long rows = (long long)qLen * (heads / kvHeads);
   sp.rowTiles = (int)((rows + rowsPerBlock - 1) / rowsPerBlock);
@@ -251,21 +253,56 @@ XaSplit planSplit(int rowsPerBlock, int keysPerStep, int blocksPerSm, int batch,
   return sp;
 }
 
+namespace {
+
+// Rows on 16-byte boundaries, and no repetition along the dimensions of which TMA takes several at once.
+bool viewAligned(const void* p, int batch, int64_t b, int tokens, int64_t t, int heads, int64_t h, bool headsTogether) {
+  return ((uintptr_t)p & 15) == 0 && (batch == 1 || b % 8 == 0) && (tokens <= 1 || (t % 8 == 0 && t != 0)) &&
+         (heads == 1 || (h % 8 == 0 && !(headsTogether && h == 0)));
+}
+bool crossAttnAligned(const CrossAttnArgs& a) {
+  return viewAligned(a.q, a.batch, a.qB, a.qLen, a.qT, a.heads, a.qH, true) && viewAligned(a.k, a.batch, a.kB, a.kLen, a.kT, a.kvHeads, a.kH, false) &&
+         viewAligned(a.v, a.batch, a.vB, a.kLen, a.vT, a.kvHeads, a.vH, false) && viewAligned(a.out, a.batch, a.oB, a.qLen, a.oT, a.heads, a.oH, true);
+}
+
+// What a call runs.  The workspace is a function of the sizes alone, so the plan is too: where the sizes suit the tensor cores and
+// only the tensors' alignment does not, the CUDA-core kernel cuts the keys as the other would.
+struct Plan {
+  bool tc;
+  int tilesPerBlock;
+  XaSplit sp;
+};
+Plan planFor(int dt, int batch, int qLen, int kLen, int heads, int kvHeads, int dq, int dv) {
+  Plan p = {};
+  p.tc = crossAttnTcSizes(dt, heads, kvHeads, dq, dv);
+  if(p.tc) p.sp = crossAttnTcSplit(batch, qLen, kLen, heads, kvHeads, dv, &p.tilesPerBlock);
+  else p.sp = xaPlanSplit(XS_ROWS, XS_KEYS, 2, batch, qLen, kLen, heads, kvHeads, dv);
+  return p;
+}
+
 }  // namespace
 
-size_t crossAttnWorkspace(int, int batch, int qLen, int kLen, int heads, int kvHeads, int, int dv) {
-  return planSplit(XS_ROWS, XS_KEYS, 2, batch, qLen, kLen, heads, kvHeads, dv).workspace;
+size_t crossAttnWorkspace(int dt, int batch, int qLen, int kLen, int heads, int kvHeads, int dq, int dv) {
+  return planFor(dt, batch, qLen, kLen, heads, kvHeads, dq, dv).sp.workspace;
 }
 
 cudaError_t launchCrossAttn(cudaStream_t st, const CrossAttnArgs& a) {
   if(a.batch == 0 || a.qLen == 0) return cudaSuccess;
-  const XaSplit sp = planSplit(XS_ROWS, XS_KEYS, 2, a.batch, a.qLen, a.kLen, a.heads, a.kvHeads, a.dv);
-  cudaError_t e;
-  switch(a.dt) {
-    case DT_F32: e = simtLaunchT<float>(st, a, sp); break;
-    case DT_F16: e = simtLaunchT<__half>(st, a, sp); break;
-    default: e = simtLaunchT<__nv_bfloat16>(st, a, sp); break;
+  Plan p = planFor(a.dt, a.batch, a.qLen, a.kLen, a.heads, a.kvHeads, a.dq, a.dv);
+  XaSplit& sp = p.sp;
+  if(p.tc && !crossAttnAligned(a)) {
+    p.tc = false;
+    sp.rowTiles = (int)(((long long)a.qLen * (a.heads / a.kvHeads) + XS_ROWS - 1) / XS_ROWS);
+    sp.blocks = (unsigned)((long long)a.batch * a.kvHeads * sp.rowTiles * sp.parts);
   }
+  cudaError_t e;
+  if(p.tc) e = launchCrossAttnTc(st, a, sp, p.tilesPerBlock);
+  else
+    switch(a.dt) {
+      case DT_F32: e = simtLaunchT<float>(st, a, sp); break;
+      case DT_F16: e = simtLaunchT<__half>(st, a, sp); break;
+      default: e = simtLaunchT<__nv_bfloat16>(st, a, sp); break;
+    }
   if(e != cudaSuccess || sp.parts == 1) return e;
   const long long rows = (long long)a.batch * a.qLen * a.heads;
   const dim3 grid((unsigned)std::min<long long>((rows + 7) / 8, 16LL * smCount()));

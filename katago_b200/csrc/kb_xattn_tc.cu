@@ -1,0 +1,410 @@
+// Attention to states of another length on the tensor cores: fp16 / bf16, head sizes up to 128 in multiples of 8, rows on 16-byte
+// boundaries.
+//
+// crossAttnTcKernel: a CTA takes one or two tiles of up to 128 rows (a key head's rows, kb_xattn.cu) and a range of keys, 128 at a
+// time.  Two warpgroups do the softmax of one row tile each, a row per thread; of the third, warp 8 requests Q, K and V by TMA,
+// warp 9 issues the MMAs, warp 10 finds out which keys of a tile are attended and clears the rows of V that are not.
+//
+//   S = Q K^T into 128 columns of tensor memory, the probabilities (16 bit, two per column) back over the same columns, O = P V with P
+//   read from tensor memory into 64 or 128 further columns.  With two row tiles the tensor pipe works on one while the other's
+//   warpgroup does its exponentials:  S0(j) | PV1(j-1) | S1(j) | PV0(j) | S0(j+1) ...
+//
+// The row maximum is kept in units of log2; p = 2^(scale log2(e) s - ref), where ref follows the maximum only when that has grown by
+// more than 8 (p stays below 2^8, sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O
+// through registers and a wait for the product before.  The factor cancels in O / sum.
+//
+// Keys that are not attended: their scores become -inf whatever they are, and their rows of V are cleared in shared memory, since 0
+// times an infinity would be a NaN.  Rows of the tile that are no tokens are computed and not written.
+//
+// What bounds it: the exponentials (16 per clock and SM: 1024 cycles for 128 x 128) beside the MMAs (1024 cycles for the
+// two products with head size 128, 512 with 64).
+#include "kb_kernels.cuh"
+#include "kb_ops.h"
+#include "kb_ops_dev.cuh"
+#include "kb_xattn.cuh"
+
+#include <algorithm>
+
+namespace kb {
+
+namespace {
+
+constexpr int XT_THREADS = 384, XT_KEYS = 128, XT_ERR = 311;
+constexpr int XT_HALF = 128 * 64 * 2;  // bytes of 128 rows x 64 channels
+constexpr float XT_GROW = 8.0f;
+
+struct CrossAttnTcArgs {
+  CrossAttnArgs x;
+  XaSplit sp;
+  int G, tileTokens, tileRows, tilesPerBlock;
+  int qUse[3], kUse[3], vUse[3];  // 0 where a tensor repeats along the batch / token / head dimension
+};
+
+// D: head size that K and V tiles are laid out for (64 or 128; both may be smaller)
+template <int D> struct XtShape {
+  static constexpr int HALVES = D / 64;
+  static constexpr int TILE = HALVES * XT_HALF;          // bytes of 128 rows
+  static constexpr int STAGES = D == 64 ? 4 : 2;         // tiles of K, and of V, in flight
+  static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + 1024 + 1024;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
+  const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const CrossAttnTcArgs a) {
+  typedef XtShape<D> Sh;
+  constexpr int ST = Sh::STAGES;
+  extern __shared__ uint8_t smemRaw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
+  uint8_t* sQ = smem;                       // [2] row tiles
+  uint8_t* sK = sQ + 2 * Sh::TILE;          // [ST]
+  uint8_t* sV = sK + ST * Sh::TILE;         // [ST]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + ST * Sh::TILE);
+  uint64_t* bQ = bars;                      // [2] a row tile has arrived
+  uint64_t* bKFull = bQ + 2;                // [ST]
+  uint64_t* bKEmpty = bKFull + ST;
+  uint64_t* bVFull = bKEmpty + ST;
+  uint64_t* bVReady = bVFull + ST;          // ... and rows of keys that are not attended are cleared; the tile's key bits are set
+  uint64_t* bVEmpty = bVReady + ST;
+  uint64_t* bS = bVEmpty + ST;              // [2] scores are complete
+  uint64_t* bP = bS + 2;                    // [2] probabilities are complete
+  uint64_t* bO = bP + 2;                    // [2] their product with V is
+  uint32_t* sBits = reinterpret_cast<uint32_t*>(bO + 2);  // [ST][4] attended keys
+  uint32_t* tmemSlot = sBits + ST * 4;
+  volatile int* abortFlag = reinterpret_cast<volatile int*>(tmemSlot + 1);
+
+  const CrossAttnArgs& x = a.x;
+  const int warp = warpIndex(), lane = threadIdx.x & 31;
+  if(threadIdx.x == 0) {
+    for(int i = 0; i < 2; i++) { mbarInit(smemU32(&bQ[i]), 1); mbarInit(smemU32(&bS[i]), 1); mbarInit(smemU32(&bP[i]), 4); mbarInit(smemU32(&bO[i]), 1); }
+    for(int i = 0; i < ST; i++) {
+      mbarInit(smemU32(&bKFull[i]), 1); mbarInit(smemU32(&bKEmpty[i]), 1);
+      mbarInit(smemU32(&bVFull[i]), 1); mbarInit(smemU32(&bVReady[i]), 1); mbarInit(smemU32(&bVEmpty[i]), 1);
+    }
+    *abortFlag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fenceProxyAsync();
+  }
+  if(warp == 9) { tmemAlloc(smemU32(tmemSlot), 512); tmemRelinquish(); }
+  tcFenceBefore();
+  __syncthreads();
+  tcFenceAfter();
+  gridDepLaunch();
+  gridDepWait();
+  const uint32_t tmem = *tmemSlot;
+  const XaBlock blk = xaBlock(x, a.sp, a.tileRows * a.tilesPerBlock);
+  const int rows = xaRows(x, blk.b, a.G), keys = xaKeys(x, blk.b);
+  const int k0 = blk.part * a.sp.chunk, k1 = (int)min((long long)keys, (long long)k0 + a.sp.chunk);
+  const bool idle = blk.row0 >= rows || (blk.part > 0 && k0 >= keys);  // part 0 reports a row without keys
+  const int nKeys = idle ? 0 : max(0, k1 - k0), nT = (nKeys + XT_KEYS - 1) / XT_KEYS;
+  const int nTiles = idle ? 0 : min(a.tilesPerBlock, (rows - blk.row0 + a.tileRows - 1) / a.tileRows);
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return opWaitInline(smemU32(bar), parity, abortFlag, x.status, XT_ERR); };
+
+  if(warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    const int qHalves = (x.dq + 63) / 64, vHalves = (x.dv + 63) / 64;
+    if(warp == 8 && nT > 0) {
+      // ---------------- requests ----------------
+      if(electOne()) {
+        const int b = blk.b, kvh = blk.kvh;
+        auto loadRows = [&](uint8_t* dst, const CUtensorMap* map, const int* use, int h, int t, int halves, uint64_t* bar) {
+          for(int i = 0; i < halves; i++) tmaLoad4d(smemU32(dst + i * XT_HALF), map, i * 64, h * use[2], t * use[1], b * use[0], smemU32(bar));
+        };
+        auto loadQ = [&](int t) {
+          mbarExpectTx(smemU32(&bQ[t]), (uint32_t)(qHalves * a.tileRows * 128));
+          loadRows(sQ + t * Sh::TILE, &tmQ, a.qUse, kvh * a.G, (blk.row0 + t * a.tileRows) / a.G, qHalves, &bQ[t]);
+        };
+        bool ok = true;
+        int kAsked = 0, vAsked = 0;
+        loadQ(0);
+        for(int j = 0; j < nT && ok; j++) {
+          const int s = j % ST;
+          const uint32_t before = (uint32_t)(j / ST - 1) & 1u;
+          if(j >= ST && !wait(&bKEmpty[s], before)) { ok = false; break; }
+          mbarExpectTx(smemU32(&bKFull[s]), (uint32_t)(qHalves * XT_HALF));
+          loadRows(sK + s * Sh::TILE, &tmK, a.kUse, kvh, k0 + j * XT_KEYS, qHalves, &bKFull[s]);
+          kAsked++;
+          if(j == 0 && nTiles > 1) loadQ(1);
+          if(j >= ST && !wait(&bVEmpty[s], before)) { ok = false; break; }
+          mbarExpectTx(smemU32(&bVFull[s]), (uint32_t)(vHalves * XT_HALF));
+          loadRows(sV + s * Sh::TILE, &tmV, a.vUse, kvh, k0 + j * XT_KEYS, vHalves, &bVFull[s]);
+          vAsked++;
+        }
+        if(!ok) {  // copies in flight land before the CTA may end
+          volatile int keepWaiting = 0;
+          for(int t = 0; t < nTiles; t++) mbarWait(smemU32(&bQ[t]), 0, &keepWaiting, 1000000ull);
+          for(int j = max(0, kAsked - ST); j < kAsked; j++) mbarWait(smemU32(&bKFull[j % ST]), (uint32_t)(j / ST) & 1u, &keepWaiting, 1000000ull);
+          for(int j = max(0, vAsked - ST); j < vAsked; j++) mbarWait(smemU32(&bVFull[j % ST]), (uint32_t)(j / ST) & 1u, &keepWaiting, 1000000ull);
+        }
+      }
+      __syncwarp();
+    }
+    else if(warp == 9 && nT > 0) {
+      // ---------------- MMAs ----------------
+      if(electOne()) {
+        const uint32_t idescS = opIdesc<T>(128, XT_KEYS), idescO = opIdesc<T>(128, D, true);
+        const int qSteps = (x.dq + 15) / 16;
+        // V is the MN-major operand: 64 channels per row of 128 bytes, 8 keys 1024 bytes apart, the second 64 channels XT_HALF on
+        auto vDescLo = [](uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | ((uint32_t)(XT_HALF >> 4) << 16); };
+        bool ok = true;
+        auto scores = [&](int t, int j) {
+          const uint32_t q = smemU32(sQ + t * Sh::TILE), k = smemU32(sK + (j % ST) * Sh::TILE);
+#pragma unroll
+          for(int i = 0; i < D / 16; i++)
+            if(i < qSteps)
+              ummaLoHi(tmem + t * 128u, opDescLo(q + (i / 4) * XT_HALF) + 2 * (i & 3), opDescLo(k + (i / 4) * XT_HALF) + 2 * (i & 3), OP_DESC_HI, idescS, i > 0 ? 1u : 0u);
+          ummaCommit(smemU32(&bS[t]));
+        };
+        auto product = [&](int t, int j) {  // false: a wait ran out
+          if(!wait(&bVReady[j % ST], (uint32_t)(j / ST) & 1u) || !wait(&bP[t], (uint32_t)j & 1u)) return false;
+          tcFenceAfter();
+          const uint32_t v = vDescLo(smemU32(sV + (j % ST) * Sh::TILE));
+#pragma unroll
+          for(int i = 0; i < XT_KEYS / 16; i++)
+            ummaTmemA(tmem + 256u + t * D, tmem + t * 128u + 8u * i, v + 128u * i, OP_DESC_HI, idescO, (j > 0 || i > 0) ? 1u : 0u);
+          ummaCommit(smemU32(&bO[t]));
+          return true;
+        };
+        ok = wait(&bQ[0], 0);
+        for(int j = 0; j < nT && ok; j++) {
+          if(!wait(&bKFull[j % ST], (uint32_t)(j / ST) & 1u)) break;
+          tcFenceAfter();
+          scores(0, j);
+          if(nTiles > 1) {
+            if(j > 0) {
+              if(!product(1, j - 1)) break;
+              ummaCommit(smemU32(&bVEmpty[(j - 1) % ST]));
+            }
+            if(j == 0 && !wait(&bQ[1], 0)) break;
+            scores(1, j);
+          }
+          ummaCommit(smemU32(&bKEmpty[j % ST]));
+          if(!product(0, j)) break;
+          if(nTiles == 1) ummaCommit(smemU32(&bVEmpty[j % ST]));
+          if(j == nT - 1 && nTiles > 1) product(1, j);
+        }
+      }
+      __syncwarp();
+    }
+    else if(warp == 10 && nT > 0) {
+      // ---------------- which keys ----------------
+      for(int j = 0; j < nT; j++) {
+        const int s = j % ST, first = k0 + j * XT_KEYS;
+        if(__any_sync(0xffffffffu, !wait(&bVFull[s], (uint32_t)(j / ST) & 1u))) break;
+        uint32_t bits[4];
+#pragma unroll
+        for(int i = 0; i < 4; i++) {
+          const int key = first + i * 32 + lane;
+          const bool on = key < k1 && (!x.keyMask || x.keyMask[(int64_t)blk.b * x.kLen + key] != 0.0f);
+          bits[i] = __ballot_sync(0xffffffffu, on);
+        }
+        if(lane < 4) sBits[s * 4 + lane] = lane == 0 ? bits[0] : (lane == 1 ? bits[1] : (lane == 2 ? bits[2] : bits[3]));
+        if((bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu) {
+          // a row of 64 channels is 128 bytes: eight lanes clear one
+          for(int i = 0; i < XT_KEYS; i += 4) {
+            const int r = i + (lane >> 3);
+            const uint32_t w = r < 32 ? bits[0] : (r < 64 ? bits[1] : (r < 96 ? bits[2] : bits[3]));
+            if(((w >> (r & 31)) & 1u) == 0u)
+              for(int h = 0; h < vHalves; h++) *reinterpret_cast<uint4*>(sV + s * Sh::TILE + h * XT_HALF + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          fenceProxyAsync();
+        }
+        __syncwarp();
+        if(lane == 0) mbarArrive(smemU32(&bVReady[s]));
+      }
+    }
+  }
+  else {
+    // ---------------- softmax: warpgroup t has row tile t, thread i of it row i ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
+    if(t < nTiles) {
+      const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+      const uint32_t tS = tmem + t * 128u + lanes, tO = tmem + 256u + t * D + lanes;
+      const float c = x.scale * 1.4426950408889634f;
+      const float2 c2 = make_float2(c, c);
+      float ref = -INFINITY, sum = 0.0f;
+      bool ok = true;
+      for(int j = 0; j < nT; j++) {
+        ok = wait(&bVReady[j % ST], (uint32_t)(j / ST) & 1u) && wait(&bS[t], (uint32_t)j & 1u);
+        if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+        tcFenceAfter();
+        // The scores leave tensor memory twice, 32 keys at a time with the next 32 in flight: once for the maximum, once for the
+        // exponentials (128 of them do not fit beside the rest in registers).
+        const uint32_t* bits = sBits + (j % ST) * 4;
+        auto leaveOut = [&](uint32_t (&s)[32], uint32_t w) {
+          if(w != 0xffffffffu) {
+#pragma unroll
+            for(int e = 0; e < 32; e++)
+              if(((w >> e) & 1u) == 0u) s[e] = 0xff800000u;
+          }
+        };
+        uint32_t s[2][32];
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmemLd32(tS, s[0]);
+        tmemLdWaitFor(s[0]);
+#pragma unroll
+        for(int i = 0; i < 4; i++) {
+          tmemLd32(tS + 32u * ((i + 1) & 3), s[(i + 1) & 1]);  // the last one is the first of the second pass
+          leaveOut(s[i & 1], bits[i]);
+#pragma unroll
+          for(int e = 0; e < 32; e++) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[i & 1][e]));
+          tmemLdWaitFor(s[(i + 1) & 1]);
+        }
+        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        const bool grow = now > ref + XT_GROW || (ref == -INFINITY && now > ref);
+        if(__any_sync(0xffffffffu, grow)) {
+          float keep = 1.0f;
+          if(grow) {
+            keep = exp2f(ref - now);
+            ref = now;
+            sum *= keep;
+          }
+          if(j > 0) {
+            ok = wait(&bO[t], (uint32_t)(j - 1) & 1u);
+            if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+            tcFenceAfter();
+#pragma unroll
+            for(int d = 0; d < D; d += 16) {
+              uint32_t o[16];
+              tmemLd16(tO + d, o);
+              tmemLdWaitFor(o);
+#pragma unroll
+              for(int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmemSt16(tO + d, o);
+            }
+          }
+        }
+        const float base = ref == -INFINITY ? 0.0f : -ref;
+        const float2 base2 = make_float2(base, base);
+        float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+        for(int i = 0; i < 4; i++) {
+          if(i < 3) tmemLd32(tS + 32u * (i + 1), s[(i + 1) & 1]);
+          leaveOut(s[i & 1], bits[i]);
+          uint32_t p[16];
+#pragma unroll
+          for(int e = 0; e < 16; e++) {
+            const float2 v = __ffma2_rn(make_float2(__uint_as_float(s[i & 1][2 * e]), __uint_as_float(s[i & 1][2 * e + 1])), c2, base2);
+            const float2 w = make_float2(ex2Approx(v.x), ex2Approx(v.y));
+            part[e & 1] = __fadd2_rn(part[e & 1], w);
+            p[e] = opPack<T>(w.x, w.y);
+          }
+          tmemSt16(tS + 16u * i, p);  // over scores of keys that have been taken out (chunk i/2)
+          if(i < 3) tmemLdWaitFor(s[(i + 1) & 1]);
+        }
+        sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
+        tmemStWait();
+        tcFenceBefore();
+        __syncwarp();
+        if(lane == 0) mbarArrive(smemU32(&bP[t]));
+      }
+      if(nT > 0 && ok) {
+        ok = wait(&bO[t], (uint32_t)(nT - 1) & 1u);
+        if(__any_sync(0xffffffffu, !ok)) ok = false;
+        tcFenceAfter();
+      }
+      const int r = blk.row0 + t * a.tileRows + row;
+      const bool mine = ok && row < a.tileRows && r < rows;
+      const int token = r / a.G, head = blk.kvh * a.G + r - token * a.G;
+      const bool live = sum != 0.0f && (!x.queryMask || (mine && x.queryMask[(int64_t)blk.b * x.qLen + token] != 0.0f));
+      const float inv = live ? 1.0f / sum : 0.0f;
+      float* part = a.sp.parts > 1 && mine ? xaPart(x, a.sp, blk, r, a.G) : nullptr;
+      T* out = (T*)x.out + blk.b * x.oB + token * x.oT + head * x.oH;
+      if(part) { part[0] = ref; part[1] = sum; }
+#pragma unroll
+      for(int d = 0; d < D; d += 32) {
+        if(d >= x.dv) break;
+        uint32_t o[32];
+        if(nT > 0) {
+          __syncwarp();
+          tmemLd32(tO + d, o);
+          tmemLdWaitFor(o);
+        }
+        else {
+#pragma unroll
+          for(int e = 0; e < 32; e++) o[e] = 0u;
+        }
+        if(!mine) continue;
+        if(part) {
+#pragma unroll
+          for(int e = 0; e < 32; e += 2)
+            if(d + e < x.dv) *reinterpret_cast<float2*>(part + 2 + d + e) = make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+        }
+        else {
+#pragma unroll
+          for(int e = 0; e < 32; e += 8)
+            if(d + e < x.dv) {
+              uint4 w = make_uint4(0u, 0u, 0u, 0u);
+              if(live) {
+                w.x = opPack<T>(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+                w.y = opPack<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+                w.z = opPack<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+                w.w = opPack<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+              }
+              *reinterpret_cast<uint4*>(out + d + e) = w;
+            }
+        }
+      }
+    }
+  }
+  tcFenceBefore();
+  __syncthreads();
+  if(warp == 9) { tcFenceAfter(); tmemDealloc(tmem, 512); }
+}
+
+// Dimensions channel, head, token, sequence; one that repeats (stride 0) is given once.
+bool encodeView(CUtensorMap* map, int* use, int dt, const void* p, int d, int heads, int tokens, int batch, int64_t sH, int64_t sT, int64_t sB, int boxHeads, int boxTokens) {
+  const int n[3] = {batch, tokens, heads};
+  const int64_t s[3] = {sB, sT, sH};
+  uint64_t dims[4] = {(uint64_t)d, 1, 1, 1}, strides[3];
+  for(int i = 0; i < 3; i++) {  // map dimension 3 - i
+    use[i] = n[i] == 1 || s[i] != 0;
+    dims[3 - i] = use[i] ? (uint64_t)n[i] : 1;
+    strides[2 - i] = n[i] > 1 && s[i] != 0 ? (uint64_t)s[i] * 2 : 16;
+  }
+  const uint32_t box[4] = {64, (uint32_t)boxHeads, (uint32_t)boxTokens, 1};
+  return encodeTiled(map, dt, p, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+template <typename T, int D> cudaError_t launchTc(cudaStream_t st, const CrossAttnTcArgs& given) {
+  CrossAttnTcArgs a = given;
+  const CrossAttnArgs& x = a.x;
+  CUtensorMap q, k, v;
+  if(!encodeView(&q, a.qUse, x.dt, x.q, x.dq, x.heads, x.qLen, x.batch, x.qH, x.qT, x.qB, a.G, a.tileTokens)) return cudaErrorInvalidValue;
+  const int kLen = std::max(1, x.kLen);
+  if(!encodeView(&k, a.kUse, x.dt, x.kLen ? x.k : x.q, x.dq, x.kvHeads, kLen, x.batch, x.kH, x.kT, x.kB, 1, XT_KEYS)) return cudaErrorInvalidValue;
+  if(!encodeView(&v, a.vUse, x.dt, x.kLen ? x.v : x.q, x.dv, x.kvHeads, kLen, x.batch, x.vH, x.vT, x.vB, 1, XT_KEYS)) return cudaErrorInvalidValue;
+  static SharedMemoryOptIn optIn;
+  const cudaError_t e = optIn((const void*)crossAttnTcKernel<T, D>, XtShape<D>::SMEM);
+  if(e != cudaSuccess) return e;
+  return launchDependent(crossAttnTcKernel<T, D>, dim3(a.sp.blocks), dim3(XT_THREADS), (size_t)XtShape<D>::SMEM, st, q, k, v, a);
+}
+
+}  // namespace
+
+bool crossAttnTcSizes(int dt, int heads, int kvHeads, int dq, int dv) {
+  return (dt == DT_F16 || dt == DT_BF16) && dq % 8 == 0 && dv % 8 == 0 && dq <= 128 && dv <= 128 && heads / kvHeads <= 128;
+}
+
+// Row tiles of a block: two where the blocks still fill the GPU, so that the tensor pipe has one while the other is in its softmax.
+XaSplit crossAttnTcSplit(int batch, int qLen, int kLen, int heads, int kvHeads, int dv, int* tilesPerBlock) {
+  const int G = heads / kvHeads, tileRows = 128 / G * G;
+  const long long rows = (long long)qLen * G, pairs = (rows + 2 * tileRows - 1) / (2 * tileRows) * batch * kvHeads;
+  *tilesPerBlock = rows > tileRows && pairs >= smCount() ? 2 : 1;
+  return xaPlanSplit(tileRows * *tilesPerBlock, XT_KEYS, 1, batch, qLen, kLen, heads, kvHeads, dv);
+}
+
+cudaError_t launchCrossAttnTc(cudaStream_t st, const CrossAttnArgs& x, const XaSplit& sp, int tilesPerBlock) {
+  CrossAttnTcArgs a = {};
+  a.x = x;
+  a.sp = sp;
+  a.G = x.heads / x.kvHeads;
+  a.tileTokens = 128 / a.G;
+  a.tileRows = a.tileTokens * a.G;
+  a.tilesPerBlock = tilesPerBlock;
+  const bool wide = x.dq > 64 || x.dv > 64;
+  if(x.dt == DT_F16) return wide ? launchTc<__half, 128>(st, a) : launchTc<__half, 64>(st, a);
+  return wide ? launchTc<__nv_bfloat16, 128>(st, a) : launchTc<__nv_bfloat16, 64>(st, a);
+}
+
+}  // namespace kb
