@@ -3,7 +3,7 @@
 //
 // crossAttnTcKernel: a CTA takes one or two tiles of up to 128 rows (a key head's rows, kb_xattn.cu) and a range of keys, 128 at a
 // time.  Two warpgroups do the softmax of one row tile each, a row per thread; of the third, warp 8 requests Q, K and V by TMA,
-// warp 9 issues the MMAs, warp 10 finds out which keys of a tile are attended and clears the rows of V that are not.
+// warp 9 issues the MMAs, warps 10 and 11 make the keys of a tile that are not attended harmless.
 //
 //   S = Q K^T into 128 columns of tensor memory, the probabilities (16 bit, two per column) back over the same columns, O = P V with P
 //   read from tensor memory into 64 or 128 further columns.  With two row tiles the tensor pipe works on one while the other's
@@ -13,8 +13,12 @@
 // more than 8 (p stays below 2^8, sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O
 // through registers and a wait for the product before.  The factor cancels in O / sum.
 //
-// Keys that are not attended: their scores become -inf whatever they are, and their rows of V are cleared in shared memory, since 0
-// times an infinity would be a NaN.  Rows of the tile that are no tokens are computed and not written.
+// Keys that are not attended (masked, or behind the last one) may hold anything.  In shared memory their rows of V are cleared and
+// their rows of K are replaced by that of an attended key of the tile: so their scores are scores of the row that lie no higher
+// than its maximum, their probabilities are finite and their products with V are 0.  Only the row's sum has to leave them out, which
+// it does by a multiplication by 1 or 0 that it makes in place of an addition; the softmax has no comparison per score.
+// (With a test of a bit per score in both passes: 341 us for 64 x 6 heads of 361 tokens over up to 2888 states, a fifth masked.)
+// Rows of the tile that are no tokens are computed and not written.
 //
 // What bounds it: the exponentials (16 per clock and SM: 1024 cycles for 128 x 128) beside the MMAs (1024 cycles for the
 // two products with head size 128, 512 with 64).
@@ -32,6 +36,7 @@ namespace {
 constexpr int XT_THREADS = 384, XT_KEYS = 128, XT_ERR = 311;
 constexpr int XT_HALF = 128 * 64 * 2;  // bytes of 128 rows x 64 channels
 constexpr float XT_GROW = 8.0f;
+enum { XT_ALL, XT_SOME, XT_NONE };
 
 struct CrossAttnTcArgs {
   CrossAttnArgs x;
@@ -45,7 +50,7 @@ template <int D> struct XtShape {
   static constexpr int HALVES = D / 64;
   static constexpr int TILE = HALVES * XT_HALF;          // bytes of 128 rows
   static constexpr int STAGES = D == 64 ? 4 : 2;         // tiles of K, and of V, in flight
-  static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + 1024 + 1024;
+  static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + STAGES * XT_KEYS * 4 + 1024 + 512;
 };
 
 template <typename T, int D>
@@ -63,13 +68,15 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
   uint64_t* bKFull = bQ + 2;                // [ST]
   uint64_t* bKEmpty = bKFull + ST;
   uint64_t* bVFull = bKEmpty + ST;
-  uint64_t* bVReady = bVFull + ST;          // ... and rows of keys that are not attended are cleared; the tile's key bits are set
+  uint64_t* bKReady = bVFull + ST;          // ... and rows of keys that are not attended are replaced
+  uint64_t* bVReady = bKReady + ST;         // ... and cleared; sKind and sCount say which they are
   uint64_t* bVEmpty = bVReady + ST;
   uint64_t* bS = bVEmpty + ST;              // [2] scores are complete
   uint64_t* bP = bS + 2;                    // [2] probabilities are complete
   uint64_t* bO = bP + 2;                    // [2] their product with V is
-  uint32_t* sBits = reinterpret_cast<uint32_t*>(bO + 2);  // [ST][4] attended keys
-  uint32_t* tmemSlot = sBits + ST * 4;
+  float* sCount = reinterpret_cast<float*>(bO + 2);   // [ST][128] 1 for an attended key, 0 for another
+  int* sKind = reinterpret_cast<int*>(sCount + ST * XT_KEYS);  // [ST] XT_ALL, XT_SOME or XT_NONE of a tile's keys are attended
+  uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(sKind + ST);
   volatile int* abortFlag = reinterpret_cast<volatile int*>(tmemSlot + 1);
 
   const CrossAttnArgs& x = a.x;
@@ -78,7 +85,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
     for(int i = 0; i < 2; i++) { mbarInit(smemU32(&bQ[i]), 1); mbarInit(smemU32(&bS[i]), 1); mbarInit(smemU32(&bP[i]), 4); mbarInit(smemU32(&bO[i]), 1); }
     for(int i = 0; i < ST; i++) {
       mbarInit(smemU32(&bKFull[i]), 1); mbarInit(smemU32(&bKEmpty[i]), 1);
-      mbarInit(smemU32(&bVFull[i]), 1); mbarInit(smemU32(&bVReady[i]), 1); mbarInit(smemU32(&bVEmpty[i]), 1);
+      mbarInit(smemU32(&bVFull[i]), 1); mbarInit(smemU32(&bKReady[i]), 1); mbarInit(smemU32(&bVReady[i]), 1); mbarInit(smemU32(&bVEmpty[i]), 1);
     }
     *abortFlag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -166,7 +173,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         };
         ok = wait(&bQ[0], 0);
         for(int j = 0; j < nT && ok; j++) {
-          if(!wait(&bKFull[j % ST], (uint32_t)(j / ST) & 1u)) break;
+          if(!wait(&bKReady[j % ST], (uint32_t)(j / ST) & 1u)) break;
           tcFenceAfter();
           scores(0, j);
           if(nTiles > 1) {
@@ -185,31 +192,53 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
       }
       __syncwarp();
     }
-    else if(warp == 10 && nT > 0) {
-      // ---------------- which keys ----------------
-      for(int j = 0; j < nT; j++) {
-        const int s = j % ST, first = k0 + j * XT_KEYS;
-        if(__any_sync(0xffffffffu, !wait(&bVFull[s], (uint32_t)(j / ST) & 1u))) break;
-        uint32_t bits[4];
+    else if(nT > 0) {
+      // ---------------- keys that are not attended: warp 10 clears V, warp 11 replaces K ----------------
+      const bool forV = warp == 10;
+      const int halves = forV ? vHalves : qHalves;
+      uint8_t* tiles = forV ? sV : sK;
+      uint64_t *full = forV ? bVFull : bKFull, *ready = forV ? bVReady : bKReady;
+      float mask[4];
+      auto fetch = [&](int j) {  // the masks of a tile, a tile ahead
 #pragma unroll
         for(int i = 0; i < 4; i++) {
-          const int key = first + i * 32 + lane;
-          const bool on = key < k1 && (!x.keyMask || x.keyMask[(int64_t)blk.b * x.kLen + key] != 0.0f);
-          bits[i] = __ballot_sync(0xffffffffu, on);
+          const int key = k0 + j * XT_KEYS + i * 32 + lane;
+          mask[i] = key < k1 ? (x.keyMask ? x.keyMask[(int64_t)blk.b * x.kLen + key] : 1.0f) : 0.0f;
         }
-        if(lane < 4) sBits[s * 4 + lane] = lane == 0 ? bits[0] : (lane == 1 ? bits[1] : (lane == 2 ? bits[2] : bits[3]));
-        if((bits[0] & bits[1] & bits[2] & bits[3]) != 0xffffffffu) {
-          // a row of 64 channels is 128 bytes: eight lanes clear one
-          for(int i = 0; i < XT_KEYS; i += 4) {
-            const int r = i + (lane >> 3);
-            const uint32_t w = r < 32 ? bits[0] : (r < 64 ? bits[1] : (r < 96 ? bits[2] : bits[3]));
-            if(((w >> (r & 31)) & 1u) == 0u)
-              for(int h = 0; h < vHalves; h++) *reinterpret_cast<uint4*>(sV + s * Sh::TILE + h * XT_HALF + r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      };
+      fetch(0);
+      for(int j = 0; j < nT; j++) {
+        const int s = j % ST;
+        uint32_t bits[4];
+#pragma unroll
+        for(int i = 0; i < 4; i++) bits[i] = __ballot_sync(0xffffffffu, mask[i] != 0.0f);
+        const bool all = (bits[0] & bits[1] & bits[2] & bits[3]) == 0xffffffffu, none = (bits[0] | bits[1] | bits[2] | bits[3]) == 0u;
+        const float count[4] = {mask[0] != 0.0f ? 1.0f : 0.0f, mask[1] != 0.0f ? 1.0f : 0.0f, mask[2] != 0.0f ? 1.0f : 0.0f, mask[3] != 0.0f ? 1.0f : 0.0f};
+        if(j + 1 < nT) fetch(j + 1);
+        if(__any_sync(0xffffffffu, !wait(&full[s], (uint32_t)(j / ST) & 1u))) break;
+        if(forV) {  // the slot's readers are done with it as long as its V is free
+          if(lane == 0) sKind[s] = all ? XT_ALL : (none ? XT_NONE : XT_SOME);
+          if(!all)
+#pragma unroll
+            for(int i = 0; i < 4; i++) sCount[s * XT_KEYS + i * 32 + lane] = count[i];
+        }
+        if(!all && (forV || !none)) {
+          const int like = bits[0] ? __ffs(bits[0]) - 1 : (bits[1] ? 31 + __ffs(bits[1]) : (bits[2] ? 63 + __ffs(bits[2]) : 95 + __ffs(bits[3])));
+          // a row of 64 channels is 128 bytes, its 16-byte pieces permuted by the row's number: eight lanes write one
+          for(int h = 0; h < halves; h++) {
+            uint8_t* tile = tiles + s * Sh::TILE + h * XT_HALF;
+            uint4 w = make_uint4(0u, 0u, 0u, 0u);
+            if(!forV) w = *reinterpret_cast<const uint4*>(tile + like * 128 + (((lane & 7) ^ (like & 7)) << 4));
+#pragma unroll
+            for(int i = 0; i < XT_KEYS; i += 4) {
+              const int r = i + (lane >> 3);
+              if(((bits[i / 32] >> (r & 31)) & 1u) == 0u) *reinterpret_cast<uint4*>(tile + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) = w;
+            }
           }
           fenceProxyAsync();
         }
         __syncwarp();
-        if(lane == 0) mbarArrive(smemU32(&bVReady[s]));
+        if(lane == 0) mbarArrive(smemU32(&ready[s]));
       }
     }
   }
@@ -230,14 +259,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         tcFenceAfter();
         // The scores leave tensor memory twice, 32 keys at a time with the next 32 in flight: once for the maximum, once for the
         // exponentials (128 of them do not fit beside the rest in registers).
-        const uint32_t* bits = sBits + (j % ST) * 4;
-        auto leaveOut = [&](uint32_t (&s)[32], uint32_t w) {
-          if(w != 0xffffffffu) {
-#pragma unroll
-            for(int e = 0; e < 32; e++)
-              if(((w >> e) & 1u) == 0u) s[e] = 0xff800000u;
-          }
-        };
+        const int kind = sKind[j % ST];
         uint32_t s[2][32];
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         tmemLd32(tS, s[0]);
@@ -245,12 +267,11 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
 #pragma unroll
         for(int i = 0; i < 4; i++) {
           tmemLd32(tS + 32u * ((i + 1) & 3), s[(i + 1) & 1]);  // the last one is the first of the second pass
-          leaveOut(s[i & 1], bits[i]);
 #pragma unroll
           for(int e = 0; e < 32; e++) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[i & 1][e]));
           tmemLdWaitFor(s[(i + 1) & 1]);
         }
-        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+        const float now = kind == XT_NONE ? -INFINITY : fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
         const bool grow = now > ref + XT_GROW || (ref == -INFINITY && now > ref);
         if(__any_sync(0xffffffffu, grow)) {
           float keep = 1.0f;
@@ -277,17 +298,33 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         const float base = ref == -INFINITY ? 0.0f : -ref;
         const float2 base2 = make_float2(base, base);
         float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+        const float4* count = reinterpret_cast<const float4*>(sCount + (j % ST) * XT_KEYS);
 #pragma unroll
         for(int i = 0; i < 4; i++) {
           if(i < 3) tmemLd32(tS + 32u * (i + 1), s[(i + 1) & 1]);
-          leaveOut(s[i & 1], bits[i]);
           uint32_t p[16];
+          if(kind == XT_NONE) {
 #pragma unroll
-          for(int e = 0; e < 16; e++) {
-            const float2 v = __ffma2_rn(make_float2(__uint_as_float(s[i & 1][2 * e]), __uint_as_float(s[i & 1][2 * e + 1])), c2, base2);
-            const float2 w = make_float2(ex2Approx(v.x), ex2Approx(v.y));
-            part[e & 1] = __fadd2_rn(part[e & 1], w);
-            p[e] = opPack<T>(w.x, w.y);
+            for(int e = 0; e < 16; e++) p[e] = 0u;
+          }
+          else {
+#pragma unroll
+            for(int e = 0; e < 32; e += 4) {
+              const float2 v0 = __ffma2_rn(make_float2(__uint_as_float(s[i & 1][e]), __uint_as_float(s[i & 1][e + 1])), c2, base2);
+              const float2 v1 = __ffma2_rn(make_float2(__uint_as_float(s[i & 1][e + 2]), __uint_as_float(s[i & 1][e + 3])), c2, base2);
+              const float2 w0 = make_float2(ex2Approx(v0.x), ex2Approx(v0.y)), w1 = make_float2(ex2Approx(v1.x), ex2Approx(v1.y));
+              if(kind == XT_ALL) {
+                part[0] = __fadd2_rn(part[0], w0);
+                part[1] = __fadd2_rn(part[1], w1);
+              }
+              else {
+                const float4 n = count[i * 8 + e / 4];
+                part[0] = __ffma2_rn(w0, make_float2(n.x, n.y), part[0]);
+                part[1] = __ffma2_rn(w1, make_float2(n.z, n.w), part[1]);
+              }
+              p[e / 2] = opPack<T>(w0.x, w0.y);
+              p[e / 2 + 1] = opPack<T>(w1.x, w1.y);
+            }
           }
           tmemSt16(tS + 16u * i, p);  // over scores of keys that have been taken out (chunk i/2)
           if(i < 3) tmemLdWaitFor(s[(i + 1) & 1]);
