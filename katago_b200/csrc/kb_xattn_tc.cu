@@ -8,6 +8,7 @@
 //   S = Q K^T into 128 columns of tensor memory, the probabilities (16 bit, two per column) back over the same columns, O = P V with P
 //   read from tensor memory into 64 or 128 further columns.  With two row tiles the tensor pipe works on one while the other's
 //   warpgroup does its exponentials:  S0(j) | PV1(j-1) | S1(j) | PV0(j) | S0(j+1) ...
+//   A block with one row tile gives the warpgroups every other tile of keys instead, and adds the two states at the end.
 //
 // The row maximum is kept in units of log2; p = 2^(scale log2(e) s - ref), where ref follows the maximum only when that has grown by
 // more than 8 (p stays below 2^8, sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O
@@ -20,8 +21,11 @@
 // (With a test of a bit per score in both passes: 341 us for 64 x 6 heads of 361 tokens over up to 2888 states, a fifth masked.)
 // Rows of the tile that are no tokens are computed and not written.
 //
-// What bounds it: the exponentials (16 per clock and SM: 1024 cycles for 128 x 128) beside the MMAs (1024 cycles for the
-// two products with head size 128, 512 with 64).
+// What bounds it: the exponentials.  The special-function units give 16 per clock and SM, 1024 cycles for 128 x 128, as long as the
+// two products of head size 128 take and twice as long as those of 64.  So a share of them (XtShape::POLY pairs of every eight) is
+// computed on the FMA units: t = n + f with n whole and |f| <= 1/2, 2^f by a polynomial, n added to the exponent's bits.  The
+// polynomials are minimax fits of the relative error over [-1/2, 1/2] (Remez exchange): degree 3 is off by 7.5e-5 at most, for
+// bf16 probabilities, whose rounding is 3.9e-3; degree 4 by 2.6e-6, for fp16 with 4.9e-4.
 #include "kb_kernels.cuh"
 #include "kb_ops.h"
 #include "kb_ops_dev.cuh"
@@ -50,8 +54,44 @@ template <int D> struct XtShape {
   static constexpr int HALVES = D / 64;
   static constexpr int TILE = HALVES * XT_HALF;          // bytes of 128 rows
   static constexpr int STAGES = D == 64 ? 4 : 2;         // tiles of K, and of V, in flight
-  static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + STAGES * XT_KEYS * 4 + 1024 + 512;
+  static constexpr int POLY = D == 64 ? 3 : 2;
+  static constexpr bool APART = D == 64;                 // probabilities have columns of their own
+  static constexpr uint32_t O_AT = 256, P_AT = APART ? 256 + 2 * D : 0, P_STEP = APART ? 64 : 128;
+  static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + STAGES * XT_KEYS * 4 + 4 * 128 * 4 + 1024 + 512;
 };
+
+__device__ __forceinline__ float max3Nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 2^t of two numbers up to some 100 on the FMA units; below -126 as for -126.  A NaN does not survive it: rows that have one get
+// a reference of NaN, which the exponentials of the special-function units carry on.
+template <typename T> __device__ __forceinline__ float2 ex2Poly(float2 t) {
+  constexpr bool LONG = std::is_same<T, __half>::value;
+  t.x = fmaxf(t.x, -126.0f);
+  t.y = fmaxf(t.y, -126.0f);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are the nearest whole number
+  const float2 r = __fadd2_rn(t, magic);
+  const float2 n = __fadd2_rn(r, make_float2(-12582912.0f, -12582912.0f));
+  const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), t);
+  auto both = [](float c) { return make_float2(c, c); };
+  float2 p;
+  if(LONG) {
+    p = __ffma2_rn(f, both(0.009570102207362652f), both(0.05591785907745361f));
+    p = __ffma2_rn(f, p, both(0.240247443318367f));
+    p = __ffma2_rn(f, p, both(0.6931217908859253f));
+    p = __ffma2_rn(f, p, both(0.9999992847442627f));
+  }
+  else {
+    p = __ffma2_rn(f, both(0.0551716685295105f), both(0.2426111251115799f));
+    p = __ffma2_rn(f, p, both(0.6932609677314758f));
+    p = __ffma2_rn(f, p, both(0.9999280571937561f));
+  }
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(r.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(r.y) << 23)));
+}
+__device__ __forceinline__ void softmaxWarpgroupsSync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
@@ -72,17 +112,19 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
   uint64_t* bVReady = bKReady + ST;         // ... and cleared; sKind and sCount say which they are
   uint64_t* bVEmpty = bVReady + ST;
   uint64_t* bS = bVEmpty + ST;              // [2] scores are complete
-  uint64_t* bP = bS + 2;                    // [2] probabilities are complete
-  uint64_t* bO = bP + 2;                    // [2] their product with V is
+  uint64_t* bRead = bS + 2;                 // [2] ... and have been read
+  uint64_t* bP = bRead + 2;                 // [2][2] probabilities of the first, the second 64 keys are complete
+  uint64_t* bO = bP + 4;                    // [2] their product with V is
   float* sCount = reinterpret_cast<float*>(bO + 2);   // [ST][128] 1 for an attended key, 0 for another
-  int* sKind = reinterpret_cast<int*>(sCount + ST * XT_KEYS);  // [ST] XT_ALL, XT_SOME or XT_NONE of a tile's keys are attended
+  float* sState = sCount + ST * XT_KEYS;              // [2][2][128] reference and sum of the rows, where their keys are cut in two
+  int* sKind = reinterpret_cast<int*>(sState + 4 * 128);  // [ST] XT_ALL, XT_SOME or XT_NONE of a tile's keys are attended
   uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(sKind + ST);
   volatile int* abortFlag = reinterpret_cast<volatile int*>(tmemSlot + 1);
 
   const CrossAttnArgs& x = a.x;
   const int warp = warpIndex(), lane = threadIdx.x & 31;
   if(threadIdx.x == 0) {
-    for(int i = 0; i < 2; i++) { mbarInit(smemU32(&bQ[i]), 1); mbarInit(smemU32(&bS[i]), 1); mbarInit(smemU32(&bP[i]), 4); mbarInit(smemU32(&bO[i]), 1); }
+    for(int i = 0; i < 2; i++) { mbarInit(smemU32(&bQ[i]), 1); mbarInit(smemU32(&bS[i]), 1); mbarInit(smemU32(&bRead[i]), 4); mbarInit(smemU32(&bP[2 * i]), 4); mbarInit(smemU32(&bP[2 * i + 1]), 4); mbarInit(smemU32(&bO[i]), 1); }
     for(int i = 0; i < ST; i++) {
       mbarInit(smemU32(&bKFull[i]), 1); mbarInit(smemU32(&bKEmpty[i]), 1);
       mbarInit(smemU32(&bVFull[i]), 1); mbarInit(smemU32(&bKReady[i]), 1); mbarInit(smemU32(&bVReady[i]), 1); mbarInit(smemU32(&bVEmpty[i]), 1);
@@ -104,6 +146,10 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
   const bool idle = blk.row0 >= rows || (blk.part > 0 && k0 >= keys);  // part 0 reports a row without keys
   const int nKeys = idle ? 0 : max(0, k1 - k0), nT = (nKeys + XT_KEYS - 1) / XT_KEYS;
   const int nTiles = idle ? 0 : min(a.tilesPerBlock, (rows - blk.row0 + a.tileRows - 1) / a.tileRows);
+  const bool cut = nTiles == 1 && nT > 1;  // one row tile: warpgroup t has key tiles t, t + 2, ...
+  const bool two = nTiles > 1 || cut;
+  const int steps0 = cut ? (nT + 1) / 2 : nT, steps1 = cut ? nT / 2 : nT;
+  auto keyTile = [&](int t, int i) { return cut ? 2 * i + t : i; };
   auto wait = [&](uint64_t* bar, uint32_t parity) { return opWaitInline(smemU32(bar), parity, abortFlag, x.status, XT_ERR); };
 
   if(warp >= 8) {
@@ -152,43 +198,52 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         const int qSteps = (x.dq + 15) / 16;
         // V is the MN-major operand: 64 channels per row of 128 bytes, 8 keys 1024 bytes apart, the second 64 channels XT_HALF on
         auto vDescLo = [](uint32_t saddr) { return ((saddr & 0x3FFFFu) >> 4) | ((uint32_t)(XT_HALF >> 4) << 16); };
-        bool ok = true;
-        auto scores = [&](int t, int j) {
-          const uint32_t q = smemU32(sQ + t * Sh::TILE), k = smemU32(sK + (j % ST) * Sh::TILE);
+        auto scores = [&](int t, int i) {
+          const int j = keyTile(t, i);
+          const uint32_t q = smemU32(sQ + (cut ? 0 : t) * Sh::TILE), k = smemU32(sK + (j % ST) * Sh::TILE);
 #pragma unroll
-          for(int i = 0; i < D / 16; i++)
-            if(i < qSteps)
-              ummaLoHi(tmem + t * 128u, opDescLo(q + (i / 4) * XT_HALF) + 2 * (i & 3), opDescLo(k + (i / 4) * XT_HALF) + 2 * (i & 3), OP_DESC_HI, idescS, i > 0 ? 1u : 0u);
+          for(int d = 0; d < D / 16; d++)
+            if(d < qSteps)
+              ummaLoHi(tmem + t * 128u, opDescLo(q + (d / 4) * XT_HALF) + 2 * (d & 3), opDescLo(k + (d / 4) * XT_HALF) + 2 * (d & 3), OP_DESC_HI, idescS, d > 0 ? 1u : 0u);
           ummaCommit(smemU32(&bS[t]));
+          if(cut || t == 1 || !two) ummaCommit(smemU32(&bKEmpty[j % ST]));
         };
-        auto product = [&](int t, int j) {  // false: a wait ran out
-          if(!wait(&bVReady[j % ST], (uint32_t)(j / ST) & 1u) || !wait(&bP[t], (uint32_t)j & 1u)) return false;
-          tcFenceAfter();
+        auto product = [&](int t, int i) {  // false: a wait ran out
+          const int j = keyTile(t, i);
+          if(!wait(&bVReady[j % ST], (uint32_t)(j / ST) & 1u)) return false;
           const uint32_t v = vDescLo(smemU32(sV + (j % ST) * Sh::TILE));
 #pragma unroll
-          for(int i = 0; i < XT_KEYS / 16; i++)
-            ummaTmemA(tmem + 256u + t * D, tmem + t * 128u + 8u * i, v + 128u * i, OP_DESC_HI, idescO, (j > 0 || i > 0) ? 1u : 0u);
+          for(int h = 0; h < 2; h++) {
+            if(!wait(&bP[2 * t + h], (uint32_t)i & 1u)) return false;
+            tcFenceAfter();
+#pragma unroll
+            for(int k = 4 * h; k < 4 * h + 4; k++)
+              ummaTmemA(tmem + Sh::O_AT + t * D, tmem + Sh::P_AT + t * Sh::P_STEP + 8u * k, v + 128u * k, OP_DESC_HI, idescO, (i > 0 || k > 0) ? 1u : 0u);
+          }
           ummaCommit(smemU32(&bO[t]));
+          if(cut || t == 1 || !two) ummaCommit(smemU32(&bVEmpty[j % ST]));
           return true;
         };
-        ok = wait(&bQ[0], 0);
-        for(int j = 0; j < nT && ok; j++) {
-          if(!wait(&bKReady[j % ST], (uint32_t)(j / ST) & 1u)) break;
+        auto nextScores = [&](int t, int i) {
+          const int j = keyTile(t, i);
+          if(!wait(&bKReady[j % ST], (uint32_t)(j / ST) & 1u)) return false;
+          if(Sh::APART && i > 0 && !wait(&bRead[t], (uint32_t)(i - 1) & 1u)) return false;
           tcFenceAfter();
-          scores(0, j);
-          if(nTiles > 1) {
-            if(j > 0) {
-              if(!product(1, j - 1)) break;
-              ummaCommit(smemU32(&bVEmpty[(j - 1) % ST]));
-            }
-            if(j == 0 && !wait(&bQ[1], 0)) break;
-            scores(1, j);
+          scores(t, i);
+          return true;
+        };
+        // Where the probabilities have columns of their own the next scores come before the product: the softmax never waits.
+        // Where they lie over the scores the next scores follow the product that reads them.
+        bool ok = wait(&bQ[0], 0) && nextScores(0, 0);
+        ok = ok && (!two || ((cut || wait(&bQ[1], 0)) && nextScores(1, 0)));
+        for(int i = 0; i < steps0 && ok; i++)
+          for(int t = 0; t < (two ? 2 : 1) && ok; t++) {
+            const int steps = t == 0 ? steps0 : steps1;
+            if(i >= steps) break;
+            if(Sh::APART && i + 1 < steps) ok = nextScores(t, i + 1);
+            ok = ok && product(t, i);
+            if(!Sh::APART && i + 1 < steps) ok = ok && nextScores(t, i + 1);
           }
-          ummaCommit(smemU32(&bKEmpty[j % ST]));
-          if(!product(0, j)) break;
-          if(nTiles == 1) ummaCommit(smemU32(&bVEmpty[j % ST]));
-          if(j == nT - 1 && nTiles > 1) product(1, j);
-        }
       }
       __syncwarp();
     }
@@ -246,33 +301,37 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
     // ---------------- softmax: warpgroup t has row tile t, thread i of it row i ----------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
-    if(t < nTiles) {
+    if(t < nTiles || cut) {
+      const int steps = t == 0 ? steps0 : steps1;
       const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-      const uint32_t tS = tmem + t * 128u + lanes, tO = tmem + 256u + t * D + lanes;
+      const uint32_t tS = tmem + t * 128u + lanes, tO = tmem + Sh::O_AT + t * D + lanes, tP = tmem + Sh::P_AT + t * Sh::P_STEP + lanes;
       const float c = x.scale * 1.4426950408889634f;
       const float2 c2 = make_float2(c, c);
       float ref = -INFINITY, sum = 0.0f;
       bool ok = true;
-      for(int j = 0; j < nT; j++) {
-        ok = wait(&bVReady[j % ST], (uint32_t)(j / ST) & 1u) && wait(&bS[t], (uint32_t)j & 1u);
+      for(int i = 0; i < steps; i++) {
+        const int j = keyTile(t, i);
+        ok = wait(&bVReady[j % ST], (uint32_t)(j / ST) & 1u) && wait(&bS[t], (uint32_t)i & 1u);
         if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
         tcFenceAfter();
-        // The scores leave tensor memory twice, 32 keys at a time with the next 32 in flight: once for the maximum, once for the
-        // exponentials (128 of them do not fit beside the rest in registers).
         const int kind = sKind[j % ST];
-        uint32_t s[2][32];
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmemLd32(tS, s[0]);
-        tmemLdWaitFor(s[0]);
+        uint32_t s[4][32];
 #pragma unroll
-        for(int i = 0; i < 4; i++) {
-          tmemLd32(tS + 32u * ((i + 1) & 3), s[(i + 1) & 1]);  // the last one is the first of the second pass
+        for(int k = 0; k < 4; k++) tmemLd32(tS + 32u * k, s[k]);
 #pragma unroll
-          for(int e = 0; e < 32; e++) top[e & 3] = fmaxf(top[e & 3], __uint_as_float(s[i & 1][e]));
-          tmemLdWaitFor(s[(i + 1) & 1]);
+        for(int k = 0; k < 4; k++) tmemLdWaitFor(s[k]);
+        if(Sh::APART) {  // the next scores may come
+          tcFenceBefore();
+          __syncwarp();
+          if(lane == 0) mbarArrive(smemU32(&bRead[t]));
         }
-        const float now = kind == XT_NONE ? -INFINITY : fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
-        const bool grow = now > ref + XT_GROW || (ref == -INFINITY && now > ref);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for(int k = 0; k < 4; k++)
+#pragma unroll
+          for(int e = 0; e < 32; e += 2) top[(e / 2) & 3] = max3Nan(top[(e / 2) & 3], __uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1]));
+        const float now = kind == XT_NONE ? -INFINITY : max3Nan(max3Nan(top[0], top[1], top[2]), top[3], top[3]) * c;
+        const bool grow = row < a.tileRows && (now > ref + XT_GROW || now != now);
         if(__any_sync(0xffffffffu, grow)) {
           float keep = 1.0f;
           if(grow) {
@@ -280,8 +339,8 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
             ref = now;
             sum *= keep;
           }
-          if(j > 0) {
-            ok = wait(&bO[t], (uint32_t)(j - 1) & 1u);
+          if(i > 0) {
+            ok = wait(&bO[t], (uint32_t)(i - 1) & 1u);
             if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
             tcFenceAfter();
 #pragma unroll
@@ -298,78 +357,105 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         const float base = ref == -INFINITY ? 0.0f : -ref;
         const float2 base2 = make_float2(base, base);
         float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-        const float4* count = reinterpret_cast<const float4*>(sCount + (j % ST) * XT_KEYS);
+        if(Sh::APART && i > 0) {  // the product before has read the probabilities that these replace
+          ok = wait(&bO[t], (uint32_t)(i - 1) & 1u);
+          if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+          tcFenceAfter();
+        }
+        // which pairs of eight take the polynomial
+        constexpr uint32_t poly = Sh::POLY == 3 ? 0x4Au : (Sh::POLY == 2 ? 0x44u : 0u);
+        auto exponentials = [&](auto some) {  // some: not every key counts
+          const float2* count = reinterpret_cast<const float2*>(sCount + (j % ST) * XT_KEYS);
 #pragma unroll
-        for(int i = 0; i < 4; i++) {
-          if(i < 3) tmemLd32(tS + 32u * (i + 1), s[(i + 1) & 1]);
-          uint32_t p[16];
-          if(kind == XT_NONE) {
+          for(int k = 0; k < 4; k++) {
+            uint32_t p[16];
 #pragma unroll
-            for(int e = 0; e < 16; e++) p[e] = 0u;
-          }
-          else {
-#pragma unroll
-            for(int e = 0; e < 32; e += 4) {
-              const float2 v0 = __ffma2_rn(make_float2(__uint_as_float(s[i & 1][e]), __uint_as_float(s[i & 1][e + 1])), c2, base2);
-              const float2 v1 = __ffma2_rn(make_float2(__uint_as_float(s[i & 1][e + 2]), __uint_as_float(s[i & 1][e + 3])), c2, base2);
-              const float2 w0 = make_float2(ex2Approx(v0.x), ex2Approx(v0.y)), w1 = make_float2(ex2Approx(v1.x), ex2Approx(v1.y));
-              if(kind == XT_ALL) {
-                part[0] = __fadd2_rn(part[0], w0);
-                part[1] = __fadd2_rn(part[1], w1);
-              }
-              else {
-                const float4 n = count[i * 8 + e / 4];
-                part[0] = __ffma2_rn(w0, make_float2(n.x, n.y), part[0]);
-                part[1] = __ffma2_rn(w1, make_float2(n.z, n.w), part[1]);
-              }
-              p[e / 2] = opPack<T>(w0.x, w0.y);
-              p[e / 2 + 1] = opPack<T>(w1.x, w1.y);
+            for(int e = 0; e < 16; e++) {
+              const float2 v = __ffma2_rn(make_float2(__uint_as_float(s[k][2 * e]), __uint_as_float(s[k][2 * e + 1])), c2, base2);
+              const float2 w = ((poly >> (e & 7)) & 1u) ? ex2Poly<T>(v) : make_float2(ex2Approx(v.x), ex2Approx(v.y));
+              part[e & 1] = decltype(some)::value ? __ffma2_rn(w, count[k * 16 + e], part[e & 1]) : __fadd2_rn(part[e & 1], w);
+              p[e] = opPack<T>(w.x, w.y);
+            }
+            tmemSt16(tP + 16u * k, p);
+            if(k & 1) {
+              tmemStWait();
+              tcFenceBefore();
+              __syncwarp();
+              if(lane == 0) mbarArrive(smemU32(&bP[2 * t + (k >> 1)]));
             }
           }
-          tmemSt16(tS + 16u * i, p);  // over scores of keys that have been taken out (chunk i/2)
-          if(i < 3) tmemLdWaitFor(s[(i + 1) & 1]);
+        };
+        if(kind == XT_ALL) exponentials(std::false_type());
+        else if(kind == XT_SOME) exponentials(std::true_type());
+        else {
+          uint32_t p[16];
+#pragma unroll
+          for(int e = 0; e < 16; e++) p[e] = 0u;
+#pragma unroll
+          for(int k = 0; k < 4; k++) tmemSt16(tP + 16u * k, p);
+          tmemStWait();
+          tcFenceBefore();
+          __syncwarp();
+          if(lane == 0) { mbarArrive(smemU32(&bP[2 * t])); mbarArrive(smemU32(&bP[2 * t + 1])); }
         }
         sum += (part[0].x + part[0].y) + (part[1].x + part[1].y);
-        tmemStWait();
-        tcFenceBefore();
-        __syncwarp();
-        if(lane == 0) mbarArrive(smemU32(&bP[t]));
       }
-      if(nT > 0 && ok) {
-        ok = wait(&bO[t], (uint32_t)(nT - 1) & 1u);
-        if(__any_sync(0xffffffffu, !ok)) ok = false;
-        tcFenceAfter();
+      float w0 = 1.0f, w1 = 0.0f;  // of the products of the two warpgroups
+      const uint32_t tO0 = cut ? tmem + Sh::O_AT + lanes : tO, tO1 = tmem + Sh::O_AT + D + lanes;
+      if(cut) {
+        sState[t * 256 + row] = ref;
+        sState[t * 256 + 128 + row] = sum;
+        softmaxWarpgroupsSync();
+        const float r0 = sState[row], r1 = sState[256 + row];
+        ref = fmaxf(r0, r1);
+        const float from = ref == -INFINITY ? 0.0f : ref;
+        w0 = exp2f(r0 - from);
+        w1 = exp2f(r1 - from);
+        sum = w0 * sState[128 + row] + w1 * sState[384 + row];
+        ok = ok && wait(&bO[0], (uint32_t)(steps0 - 1) & 1u) && wait(&bO[1], (uint32_t)(steps1 - 1) & 1u);
       }
-      const int r = blk.row0 + t * a.tileRows + row;
+      else if(nT > 0) ok = ok && wait(&bO[t], (uint32_t)(nT - 1) & 1u);
+      if(__any_sync(0xffffffffu, !ok)) ok = false;
+      tcFenceAfter();
+      const int r = blk.row0 + (cut ? 0 : t) * a.tileRows + row;
       const bool mine = ok && row < a.tileRows && r < rows;
       const int token = r / a.G, head = blk.kvh * a.G + r - token * a.G;
-      const bool live = sum != 0.0f && (!x.queryMask || (mine && x.queryMask[(int64_t)blk.b * x.qLen + token] != 0.0f));
+      const bool live = ref != -INFINITY && sum != 0.0f && (!x.queryMask || (mine && x.queryMask[(int64_t)blk.b * x.qLen + token] != 0.0f));
       const float inv = live ? 1.0f / sum : 0.0f;
       float* part = a.sp.parts > 1 && mine ? xaPart(x, a.sp, blk, r, a.G) : nullptr;
       T* out = (T*)x.out + blk.b * x.oB + token * x.oT + head * x.oH;
-      if(part) { part[0] = ref; part[1] = sum; }
+      if(part && (t == 0 || !cut)) { part[0] = ref; part[1] = sum; }
 #pragma unroll
-      for(int d = 0; d < D; d += 32) {
+      for(int dd = 0; dd < D; dd += 16) {
+        if(cut && dd >= D / 2) break;
+        const int d = cut ? t * (D / 2) + dd : dd;  // cut: each warpgroup writes half of the channels
         if(d >= x.dv) break;
-        uint32_t o[32];
+        uint32_t o[16];
         if(nT > 0) {
           __syncwarp();
-          tmemLd32(tO + d, o);
+          tmemLd16(tO0 + d, o);
           tmemLdWaitFor(o);
+          if(cut) {
+            uint32_t o1[16];
+            tmemLd16(tO1 + d, o1);
+            tmemLdWaitFor(o1);
+#pragma unroll
+            for(int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * w0 + __uint_as_float(o1[e]) * w1);
+          }
         }
         else {
 #pragma unroll
-          for(int e = 0; e < 32; e++) o[e] = 0u;
+          for(int e = 0; e < 16; e++) o[e] = 0u;
         }
         if(!mine) continue;
         if(part) {
 #pragma unroll
-          for(int e = 0; e < 32; e += 2)
+          for(int e = 0; e < 16; e += 2)
             if(d + e < x.dv) *reinterpret_cast<float2*>(part + 2 + d + e) = make_float2(__uint_as_float(o[e]), __uint_as_float(o[e + 1]));
         }
         else {
 #pragma unroll
-          for(int e = 0; e < 32; e += 8)
+          for(int e = 0; e < 16; e += 8)
             if(d + e < x.dv) {
               uint4 w = make_uint4(0u, 0u, 0u, 0u);
               if(live) {
