@@ -36,11 +36,22 @@ __device__ __forceinline__ unsigned long long turnFraction(float freq) {
   return 2ull * (unsigned long long)__double2ll_rn(frac * 9223372036854775808.0);
 }
 
+// Turn fractions that a block keeps in shared memory; more of them (many tables of many axes) are computed where they are used.
+constexpr int ROPE_TABLE = 4096;
+
 // MODE 0: scalar pairs (any alignment), 1: V elements = V/2 adjacent pairs per access, 2: halves, V pairs per two accesses
 template <typename T, int MODE, int V>
-__global__ void __launch_bounds__(256) ropeAxesKernel(const RopeArgs a, int chunks, int rotChunks, int headsPerItem, int headGroups, long long items) {
+__global__ void __launch_bounds__(256) ropeAxesKernel(const RopeArgs a, int chunks, int rotChunks, int headsPerItem, long long items) {
+  extern __shared__ unsigned long long sTurn[];  // [freqHeads][pairs][axes], or nothing
   gridDepLaunch();
   gridDepWait();
+  const int entries = a.freqHeads * (a.rot / 2) * a.axes;
+  const bool table = entries <= ROPE_TABLE;
+  if(table) {
+    // the conversion of a frequency takes some ten fp64 operations: once per block, not once per token
+    for(int i = threadIdx.x; i < entries; i += 256) sTurn[i] = isfinite(a.freqs[i]) ? turnFraction(a.freqs[i]) : 0;
+    __syncthreads();
+  }
   constexpr int P = MODE == 0 ? 1 : (MODE == 1 ? V / 2 : V);
   const int pairs = a.rot / 2;
   const int totalHeads = a.q.heads + a.k.heads;
@@ -70,22 +81,28 @@ __global__ void __launch_bounds__(256) ropeAxesKernel(const RopeArgs a, int chun
       continue;
     }
     float cs[P], sn[P];
-    int table = -1;
+    int have = -1;  // the table whose angles they are
     const int32_t* pos = a.positions + b * a.posB + (long long)t * a.axes;
     auto angles = [&](int th) {
-      table = th;
-      const float* f = a.freqs + ((size_t)th * pairs + (size_t)c * P) * a.axes;
+      have = th;
+      const int first = (th * pairs + c * P) * a.axes;
+      unsigned long long turn[P];
+      bool finite[P];
+#pragma unroll
+      for(int p = 0; p < P; p++) { turn[p] = 0; finite[p] = true; }
+      for(int x = 0; x < a.axes; x++) {
+        const unsigned long long at = (unsigned long long)(long long)pos[x];
+#pragma unroll
+        for(int p = 0; p < P; p++) {
+          const float f = a.freqs[first + p * a.axes + x];
+          finite[p] = finite[p] && isfinite(f);
+          turn[p] += at * (table ? sTurn[first + p * a.axes + x] : turnFraction(finite[p] ? f : 0.0f));
+        }
+      }
 #pragma unroll
       for(int p = 0; p < P; p++) {
-        unsigned long long turn = 0;
-        bool finite = true;
-        for(int x = 0; x < a.axes; x++) {
-          const float fr = f[p * a.axes + x];
-          finite = finite && isfinite(fr);
-          turn += turnFraction(fr) * (unsigned long long)(long long)pos[x];
-        }
         // upper 32 bits as a signed fraction: units of half a turn for sincospif
-        const float halfTurns = finite ? (float)(int)(turn >> 32) * 4.656612873077393e-10f : __int_as_float(0x7fffffff);
+        const float halfTurns = finite[p] ? (float)(int)(turn[p] >> 32) * 4.656612873077393e-10f : __int_as_float(0x7fffffff);
         sincospif(halfTurns, &sn[p], &cs[p]);
       }
     };
@@ -110,7 +127,7 @@ __global__ void __launch_bounds__(256) ropeAxesKernel(const RopeArgs a, int chun
       for(int u = 0; u < U; u++) {
         if(hb + u >= h1) break;
         const int th = tableOf(hb + u);
-        if(th != table) angles(th);
+        if(th != have) angles(th);
 #pragma unroll
         for(int p = 0; p < P; p++) {
           T& r0 = MODE == 1 ? v[u][0].e[(2 * p) % W] : v[u][0].e[p % W];
@@ -146,13 +163,16 @@ template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a)
   // heads that one thread walks through: all of them (one set of angles), unless the threads would not fill the GPU
   const long long want = 2048LL * smCount();
   const int groups = (int)std::min<long long>(heads, std::max<long long>(1, want / perHead));
-  const int headsPerItem = (heads + groups - 1) / groups, headGroups = (heads + headsPerItem - 1) / headsPerItem;
-  const long long items = perHead * headGroups;
-  const long long blocks = std::min<long long>((items + 255) / 256, 1LL << 30);
+  const int headsPerItem = (heads + groups - 1) / groups;
+  const long long items = perHead * ((heads + headsPerItem - 1) / headsPerItem);
+  const int entries = a.freqHeads * (a.rot / 2) * a.axes;
+  const size_t smem = entries <= ROPE_TABLE ? (size_t)entries * 8 : 0;
+  // as many blocks as are resident at once walk over the items, so that each converts the frequencies once
+  const long long blocks = std::min<long long>((items + 255) / 256, 4LL * smCount());
   const dim3 grid((unsigned)blocks), block(256);
-  if(!vec) return launchDependent(ropeAxesKernel<T, 0, 1>, grid, block, 0, st, a, chunks, rotChunks, headsPerItem, headGroups, items);
-  if(a.halves) return launchDependent(ropeAxesKernel<T, 2, V>, grid, block, 0, st, a, chunks, rotChunks, headsPerItem, headGroups, items);
-  return launchDependent(ropeAxesKernel<T, 1, V>, grid, block, 0, st, a, chunks, rotChunks, headsPerItem, headGroups, items);
+  if(!vec) return launchDependent(ropeAxesKernel<T, 0, 1>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
+  if(a.halves) return launchDependent(ropeAxesKernel<T, 2, V>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
+  return launchDependent(ropeAxesKernel<T, 1, V>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
 }
 
 }  // namespace
