@@ -6,6 +6,12 @@
 //                    outputs use the packed fp32 instructions (two IEEE operations per issue slot).
 // matmulFewKernel    up to eight rows: memory-bound, the weights are read once.  A block has four weight rows and cuts K
 //                    over its warps, whose sums are added in warp order.
+// matmulFewMmaKernel the same for up to 16 rows of 16-bit types and K up to 1024, where a launch's latency is what counts.
+//                    mma.sync takes 16 weight rows against 8 rows of x.  Operands go from memory to registers, 16 bytes
+//                    per lane: the sum over K may be taken in any order, so the lane that has channels 8t..8t+7 of a weight row
+//                    feeds them as four pairs wherever the instruction wants pairs, and the lane of a row of x does the same.
+//                    4 x 1024 x 384 bf16: 2.1 us, 4.0 us in kb_matmul_tc.cu; the two meet at 4 x 16384 x 512 (4.9 us), and longer
+//                    sums are better off with asynchronous copies (4 x 4096 x 4096: 12.8 us here, 9.2 us there).
 #include "kb_kernels.cuh"
 #include "kb_ops.h"
 #include "kb_ops_dev.cuh"
@@ -166,6 +172,75 @@ __global__ void __launch_bounds__(256) matmulFewKernel(const MatmulArgs a) {
   }
 }
 
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if(std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// R8: groups of eight rows of x
+template <typename T, int R8>
+__global__ void __launch_bounds__(256) matmulFewMmaKernel(const MatmulArgs a) {
+  __shared__ float part[8][R8][4][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int n0 = blockIdx.x * 16;
+  const T* w0 = (const T*)a.w + (int64_t)min(n0 + g, a.N - 1) * a.ldw;
+  const T* w1 = (const T*)a.w + (int64_t)min(n0 + g + 8, a.N - 1) * a.ldw;
+  float acc[R8][4];
+#pragma unroll
+  for(int r = 0; r < R8; r++)
+#pragma unroll
+    for(int e = 0; e < 4; e++) acc[r][e] = 0.0f;
+  gridDepLaunch();
+  gridDepWait();
+  constexpr int U = 4;  // steps of 32 channels in flight
+  for(int kb = warp * 32 + t * 8; kb - t * 8 < a.K; kb += 256 * U) {
+    uint4 wa[U], wb[U], xv[U][R8];
+    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+    for(int u = 0; u < U; u++) {
+      const int k = kb + 256 * u;
+      const bool in = k < a.K;
+      wa[u] = in ? *reinterpret_cast<const uint4*>(w0 + k) : zero;
+      wb[u] = in ? *reinterpret_cast<const uint4*>(w1 + k) : zero;
+#pragma unroll
+      for(int r = 0; r < R8; r++)
+        xv[u][r] = in && r * 8 + g < a.M ? *reinterpret_cast<const uint4*>((const T*)a.x + (int64_t)(r * 8 + g) * a.ldx + k) : zero;
+    }
+#pragma unroll
+    for(int u = 0; u < U; u++)
+#pragma unroll
+      for(int r = 0; r < R8; r++) {
+        mma16816<T>(acc[r], wa[u].x, wb[u].x, wa[u].y, wb[u].y, xv[u][r].x, xv[u][r].y);
+        mma16816<T>(acc[r], wa[u].z, wb[u].z, wa[u].w, wb[u].w, xv[u][r].z, xv[u][r].w);
+      }
+  }
+#pragma unroll
+  for(int r = 0; r < R8; r++)
+#pragma unroll
+    for(int e = 0; e < 4; e++) part[warp][r][e][lane] = acc[r][e];
+  __syncthreads();
+  for(int i = threadIdx.x; i < R8 * 128; i += 256) {
+    // output (row of x, weight row): value e of the lane that has them
+    const int n = i & 15, m8 = (i >> 4) & 7, r = i >> 7;
+    const int e = (n >> 3) * 2 + (m8 & 1), l = (n & 7) * 4 + (m8 >> 1);
+    float v = 0.0f;
+#pragma unroll
+    for(int s = 0; s < 8; s++) v += part[s][r][e][l];
+    const int m = r * 8 + m8;
+    if(m < a.M && n0 + n < a.N) matmulStore<T>(a, m, n0 + n, v);
+  }
+}
+
+template <typename T> cudaError_t matmulFewMma(cudaStream_t st, const MatmulArgs& a) {
+  const dim3 grid((a.N + 15) / 16), block(256);
+  if(a.M <= 8) return launchDependent(matmulFewMmaKernel<T, 1>, grid, block, 0, st, a);
+  return launchDependent(matmulFewMmaKernel<T, 2>, grid, block, 0, st, a);
+}
+
 template <typename T, int V> cudaError_t matmulLaunch(cudaStream_t st, const MatmulArgs& a) {
   if(a.M <= 8) {
     const dim3 grid((a.N + FEW_COLS - 1) / FEW_COLS), block(256);
@@ -191,7 +266,10 @@ template <typename T> cudaError_t matmulLaunchT(cudaStream_t st, const MatmulArg
 }  // namespace
 
 cudaError_t launchMatmul(cudaStream_t st, const MatmulArgs& a) {
-  if(a.M > 8 && matmulTcEligible(a)) return launchMatmulTc(st, a);
+  if(matmulTcEligible(a)) {
+    if(a.M <= 16 && a.K % 8 == 0 && a.K <= 1024 && a.N <= 8192) return a.dt == DT_F16 ? matmulFewMma<__half>(st, a) : matmulFewMma<__nv_bfloat16>(st, a);
+    return launchMatmulTc(st, a);
+  }
   switch(a.dt) {
     case DT_F32: return matmulLaunchT<float>(st, a);
     case DT_F16: return matmulLaunchT<__half>(st, a);

@@ -41,7 +41,7 @@ constexpr int ROPE_TABLE = 4096;
 
 // MODE 0: scalar pairs (any alignment), 1: V elements = V/2 adjacent pairs per access, 2: halves, V pairs per two accesses
 template <typename T, int MODE, int V>
-__global__ void __launch_bounds__(256) ropeAxesKernel(const RopeArgs a, int chunks, int rotChunks, int headsPerItem, long long items) {
+__global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const RopeArgs a, int chunks, int rotChunks, int headsPerItem, long long items) {
   extern __shared__ unsigned long long sTurn[];  // [freqHeads][pairs][axes], or nothing
   gridDepLaunch();
   gridDepWait();
@@ -167,8 +167,11 @@ template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a)
   const long long items = perHead * ((heads + headsPerItem - 1) / headsPerItem);
   const int entries = a.freqHeads * (a.rot / 2) * a.axes;
   const size_t smem = entries <= ROPE_TABLE ? (size_t)entries * 8 : 0;
-  // as many blocks as are resident at once walk over the items, so that each converts the frequencies once
-  const long long blocks = std::min<long long>((items + 255) / 256, 4LL * smCount());
+  // Few blocks walk over the items, so that each converts the frequencies once.  Of 2 to 64 blocks per SM six were best: 128 x 361
+  // tokens of 12 heads of 64 (fp16, 142 MB) 28.2 us, 36 us with as many as are resident.  So were four resident blocks for
+  // adjacent pairs (34.7 us with two) and two for halves, which need their registers (2 x 20 280 tokens of 32 heads of 128, bf16,
+  // 664 MB: 124 us, 5.4 TB/s; 303 us with three, spilled).
+  const long long blocks = std::min<long long>((items + 255) / 256, 6LL * smCount());
   const dim3 grid((unsigned)blocks), block(256);
   if(!vec) return launchDependent(ropeAxesKernel<T, 0, 1>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
   if(a.halves) return launchDependent(ropeAxesKernel<T, 2, V>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
