@@ -1,9 +1,12 @@
 // y = act(x w^T + bias) + residual on a caller's own matrices, on the CUDA cores: fp32, and 16-bit matrices whose rows do not
 // start on the boundaries that TMA needs.  (16-bit matrices with aligned rows: kb_matmul_tc.cu.)
 //
-// matmulTileKernel   one tile of BM x BN outputs per block, 16 elements of K staged at a time in fp32, double-buffered: the
-//                    next slice travels through registers while this one is multiplied.  FMA-bound; pairs of neighbouring
-//                    outputs use the packed fp32 instructions (two IEEE operations per issue slot).
+// matmulF32Kernel    fp32: one tile of BM x BN outputs per block, slices of 32 channels through three stages of asynchronous copies
+//                    (16 bytes, or 4 where rows lie anywhere).  FMA-bound.  A thread reads four channels of a row at a time and
+//                    sums even and odd channels apart with the packed fp32 instructions (two IEEE operations per issue slot, no
+//                    operand has to be doubled); the two are added at the end.
+// matmulTileKernel   16-bit rows on other than 16-byte boundaries: the same tiles, converted to fp32 while they are staged; the next
+//                    slice travels through registers while this one is multiplied.
 // matmulFewKernel    up to eight rows: memory-bound, the weights are read once.  A block has four weight rows and cuts K
 //                    over its warps, whose sums are added in warp order.
 // matmulFewMmaKernel the same for up to 16 rows of 16-bit types and K up to 1024, where a launch's latency is what counts.
@@ -28,6 +31,109 @@ __device__ __forceinline__ void matmulStore(const MatmulArgs& a, int m, int n, f
   v = opAct<T>(v, a.act);
   if(a.residual) v += OpType<T>::to(((const T*)a.residual)[(int64_t)m * a.ldr + n]);
   ((T*)a.y)[(int64_t)m * a.ldy + n] = OpType<T>::from(v);
+}
+
+// VEC: rows on 16-byte boundaries and K in whole vectors.  KG: groups of 256 threads that share a slice's channels, their sums added
+// in order at the end: a tile alone on its SM needs more than eight warps to cover the latency of its shared-memory loads
+// (1083 x 362 x 361: 26 us with one group).
+template <int BM, int BN, bool VEC, int KG>
+__global__ void __launch_bounds__(256 * KG) matmulF32Kernel(const MatmulArgs a) {
+  constexpr int BK = 32, PITCH = BK + 4, STAGES = 3, TM = BM / 16, TN = BN / 16;  // 8 rows of 144 bytes start in 8 different bank groups
+  extern __shared__ float4 smem4[];
+  float* sm = reinterpret_cast<float*>(smem4);
+  const int tid = threadIdx.x, kg = tid >> 8;
+  const int tx = ((tid >> 5) & 1) * 8 + (tid & 7), ty = ((tid & 255) >> 6) * 4 + ((tid >> 3) & 3);  // a warp: four rows by eight columns
+  const int tilesN = (a.N + BN - 1) / BN;
+  const int m0 = (int)(blockIdx.x / tilesN) * BM, n0 = (int)(blockIdx.x % tilesN) * BN;
+  const float* x = (const float*)a.x;
+  const float* w = (const float*)a.w;
+  gridDepLaunch();
+  gridDepWait();
+  const int steps = (a.K + BK - 1) / BK;
+  auto load = [&](int s) {
+    float* dst = sm + (s % STAGES) * (BM + BN) * PITCH;
+    constexpr int E = VEC ? 4 : 1, PER = BK / E;
+#pragma unroll
+    for(int i = tid; i < (BM + BN) * PER; i += 256 * KG) {
+      const int r = i / PER, k = s * BK + (i % PER) * E;
+      const bool isX = r < BM;
+      const int row = isX ? m0 + r : n0 + r - BM;
+      const bool in = k < a.K && row < (isX ? a.M : a.N);
+      const float* src = in ? (isX ? x + (int64_t)row * a.ldx : w + (int64_t)row * a.ldw) + k : x;
+      const uint32_t to = smemU32(dst + r * PITCH + (i % PER) * E);
+      if(VEC) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(in ? 16 : 0) : "memory");
+      else asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(src), "r"(in ? 4 : 0) : "memory");
+    }
+  };
+  float2 acc[TM][TN];
+#pragma unroll
+  for(int i = 0; i < TM; i++)
+#pragma unroll
+    for(int j = 0; j < TN; j++) acc[i][j] = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for(int s = 0; s < STAGES - 1; s++) {
+    if(s < steps) load(s);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  for(int s = 0; s < steps; s++) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    __syncthreads();  // slice s is there, and everyone is done with the slot of slice s - 1
+    if(s + STAGES - 1 < steps) load(s + STAGES - 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const float* sA = sm + (s % STAGES) * (BM + BN) * PITCH + ty * PITCH;
+    const float* sB = sm + (s % STAGES) * (BM + BN) * PITCH + (BM + tx) * PITCH;
+    // the operands of four channels are loaded while those before are multiplied, if there are registers for both
+    constexpr int AHEAD = TM * TN <= 32 ? 1 : 0;
+    float4 av[1 + AHEAD][TM], bv[1 + AHEAD][TN];
+    auto operands = [&](int b, int k) {
+#pragma unroll
+      for(int i = 0; i < TM; i++) av[b][i] = *reinterpret_cast<const float4*>(sA + 16 * i * PITCH + k);
+#pragma unroll
+      for(int j = 0; j < TN; j++) bv[b][j] = *reinterpret_cast<const float4*>(sB + 16 * j * PITCH + k);
+    };
+    if(AHEAD) operands(0, kg * (BK / KG));
+#pragma unroll
+    for(int k = 0; k < BK / KG; k += 4) {
+      const int b = AHEAD ? (k / 4) & 1 : 0;
+      if(!AHEAD) operands(0, kg * (BK / KG) + k);
+      else if(k + 4 < BK / KG) operands((b ^ 1) * AHEAD, kg * (BK / KG) + k + 4);
+#pragma unroll
+      for(int i = 0; i < TM; i++)
+#pragma unroll
+        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(make_float2(av[b][i].x, av[b][i].y), make_float2(bv[b][j].x, bv[b][j].y), acc[i][j]);
+#pragma unroll
+      for(int i = 0; i < TM; i++)
+#pragma unroll
+        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(make_float2(av[b][i].z, av[b][i].w), make_float2(bv[b][j].z, bv[b][j].w), acc[i][j]);
+    }
+  }
+  if(KG > 1) {
+    static_assert((KG - 1) * TM * TN * 256 <= STAGES * (BM + BN) * PITCH, "the groups' sums take the place of the slices");
+    __syncthreads();
+    if(kg > 0)
+#pragma unroll
+      for(int i = 0; i < TM; i++)
+#pragma unroll
+        for(int j = 0; j < TN; j++) sm[(((kg - 1) * TM + i) * TN + j) * 256 + (tid & 255)] = acc[i][j].x + acc[i][j].y;
+    __syncthreads();
+    if(kg > 0) return;
+#pragma unroll
+    for(int g = 0; g < KG - 1; g++)
+#pragma unroll
+      for(int i = 0; i < TM; i++)
+#pragma unroll
+        for(int j = 0; j < TN; j++) acc[i][j].x += sm[((g * TM + i) * TN + j) * 256 + tid];
+  }
+#pragma unroll
+  for(int i = 0; i < TM; i++) {
+    const int m = m0 + ty + 16 * i;
+    if(m >= a.M) continue;
+#pragma unroll
+    for(int j = 0; j < TN; j++) {
+      const int n = n0 + tx + 16 * j;
+      if(n < a.N) matmulStore<float>(a, m, n, acc[i][j].x + acc[i][j].y);
+    }
+  }
 }
 
 // V: elements of K per global access
@@ -75,13 +181,14 @@ __global__ void __launch_bounds__(256) matmulTileKernel(const MatmulArgs a) {
 #pragma unroll
         for(int e = 0; e < V; e++) sB[s][lk + e][lr + i * ROWS] = OpType<T>::to(rb[i].e[e]);
   };
-  // thread (ty, tx): rows ty*4.. of every 64, columns tx*4.. of every 64 (TM and TN are multiples of 4, or the tile is 32 wide: 2)
-  constexpr int CM = TM >= 4 ? 4 : TM, CN = TN >= 4 ? 4 : TN;
-  float2 acc[TM][TN / 2];
+  // thread (ty, tx): rows ty*4.. of every 64 (or ty*TM..), columns tx*4.. of every 64, or tx, tx + 16, ...
+  constexpr int CM = TM >= 4 ? 4 : TM, CN = TN % 4 == 0 ? 4 : 1;
+  auto col = [&](int j) { return (j / CN) * 16 * CN + tx * CN + j % CN; };
+  float2 acc[TM / 2][TN];  // pairs of rows
 #pragma unroll
-  for(int i = 0; i < TM; i++)
+  for(int i = 0; i < TM / 2; i++)
 #pragma unroll
-    for(int j = 0; j < TN / 2; j++) acc[i][j] = make_float2(0.0f, 0.0f);
+    for(int j = 0; j < TN; j++) acc[i][j] = make_float2(0.0f, 0.0f);
   const int steps = (a.K + BK - 1) / BK;
   fetch(0);
   stage(0);
@@ -91,20 +198,31 @@ __global__ void __launch_bounds__(256) matmulTileKernel(const MatmulArgs a) {
     const int cur = s & 1;
 #pragma unroll
     for(int k = 0; k < BK; k++) {
-      float av[TM];
-      float2 bv[TN / 2];
+      float2 av[TM / 2];
+      float bv[TN];
 #pragma unroll
-      for(int i = 0; i < TM / CM; i++)
+      for(int i = 0; i < TM / CM; i++) {
+        const float* p = &sA[cur][k][i * 16 * CM + ty * CM];
+        if(CM == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p);
+          av[i * 2] = make_float2(v.x, v.y);
+          av[(i * 2 + 1) % (TM / 2)] = make_float2(v.z, v.w);
+        }
+        else av[i] = *reinterpret_cast<const float2*>(p);
+      }
 #pragma unroll
-        for(int e = 0; e < CM; e++) av[i * CM + e] = sA[cur][k][i * 16 * CM + ty * CM + e];
+      for(int j = 0; j < TN / CN; j++) {
+        const float* p = &sB[cur][k][j * 16 * CN + tx * CN];
+        if(CN == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(p);
+          bv[j * CN] = v.x; bv[(j * CN + 1) % TN] = v.y; bv[(j * CN + 2) % TN] = v.z; bv[(j * CN + 3) % TN] = v.w;
+        }
+        else bv[j] = *p;
+      }
 #pragma unroll
-      for(int j = 0; j < TN / CN; j++)
+      for(int i = 0; i < TM / 2; i++)
 #pragma unroll
-        for(int e = 0; e < CN / 2; e++) bv[j * (CN / 2) + e] = *reinterpret_cast<const float2*>(&sB[cur][k][j * 16 * CN + tx * CN + 2 * e]);
-#pragma unroll
-      for(int i = 0; i < TM; i++)
-#pragma unroll
-        for(int j = 0; j < TN / 2; j++) acc[i][j] = __ffma2_rn(make_float2(av[i], av[i]), bv[j], acc[i][j]);
+        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(av[i], make_float2(bv[j], bv[j]), acc[i][j]);
     }
     if(s + 1 < steps) stage(cur ^ 1);
     __syncthreads();
@@ -115,8 +233,8 @@ __global__ void __launch_bounds__(256) matmulTileKernel(const MatmulArgs a) {
     if(m >= a.M) continue;
 #pragma unroll
     for(int j = 0; j < TN; j++) {
-      const int n = n0 + (j / CN) * 16 * CN + tx * CN + j % CN;
-      if(n < a.N) matmulStore<T>(a, m, n, j % 2 == 0 ? acc[i][j / 2].x : acc[i][j / 2].y);
+      const int n = n0 + col(j);
+      if(n < a.N) matmulStore<T>(a, m, n, i % 2 == 0 ? acc[i / 2][j].x : acc[i / 2][j].y);
     }
   }
 }
@@ -241,6 +359,48 @@ template <typename T> cudaError_t matmulFewMma(cudaStream_t st, const MatmulArgs
   return launchDependent(matmulFewMmaKernel<T, 2>, grid, block, 0, st, a);
 }
 
+// The tile whose share of the SM with the most of them costs the least; the smaller ones load more operands per FMA.
+struct TileForm {
+  int bm, bn;
+  double per;  // cost of an output, relative
+  void (*run)(const MatmulArgs);
+  int threads;
+};
+template <int N> cudaError_t launchTiles(cudaStream_t st, const MatmulArgs& a, const TileForm (&forms)[N], SharedMemoryOptIn (&optIn)[N], size_t (*smem)(int, int)) {
+  int pick = 0;
+  double best = 0;
+  long long count = 0;
+  for(int i = 0; i < N; i++) {
+    const long long tiles = ((long long)a.M + forms[i].bm - 1) / forms[i].bm * ((a.N + forms[i].bn - 1) / forms[i].bn);
+    const double cost = (double)((tiles + smCount() - 1) / smCount()) * forms[i].bm * forms[i].bn * forms[i].per;
+    if(i == 0 || cost < best) { best = cost; pick = i; count = tiles; }
+  }
+  if(count >= 1LL << 31) return cudaErrorInvalidValue;
+  const size_t bytes = smem(forms[pick].bm, forms[pick].bn);
+  if(bytes > 48 * 1024) {
+    const cudaError_t e = optIn[pick]((const void*)forms[pick].run, (int)bytes);
+    if(e != cudaSuccess) return e;
+  }
+  return launchDependent(forms[pick].run, dim3((unsigned)count), dim3(forms[pick].threads), bytes, st, a);
+}
+template <typename T, int V> struct TileForms {
+  static cudaError_t launch(cudaStream_t st, const MatmulArgs& a) {
+    constexpr int VT = V > 4 ? 4 : V;  // elements of an access: four threads per staged row
+    static const TileForm forms[] = {{128, 128, 1.0, matmulTileKernel<T, 128, 128, VT>, 256}, {64, 64, 1.25, matmulTileKernel<T, 64, 64, VT>, 256},
+                                     {64, 48, 1.3, matmulTileKernel<T, 64, 48, VT>, 256}, {32, 32, 2.0, matmulTileKernel<T, 32, 32, VT>, 256}};
+    static SharedMemoryOptIn optIn[4];
+    return launchTiles(st, a, forms, optIn, [](int, int) -> size_t { return 0; });
+  }
+};
+template <int V> struct TileForms<float, V> {
+  static cudaError_t launch(cudaStream_t st, const MatmulArgs& a) {
+    static const TileForm forms[] = {{128, 128, 1.0, matmulF32Kernel<128, 128, V == 4, 1>, 256}, {128, 64, 1.15, matmulF32Kernel<128, 64, V == 4, 1>, 256}, 
+                                     {64, 64, 1.3, matmulF32Kernel<64, 64, V == 4, 2>, 512},                                     {64, 48, 1.35, matmulF32Kernel<64, 48, V == 4, 4>, 1024}, {32, 32, 1.9, matmulF32Kernel<32, 32, V == 4, 4>, 1024}};
+    static SharedMemoryOptIn optIn[5];
+    return launchTiles(st, a, forms, optIn, [](int bm, int bn) -> size_t { return (size_t)3 * (bm + bn) * 36 * 4; });
+  }
+};
+
 template <typename T, int V> cudaError_t matmulLaunch(cudaStream_t st, const MatmulArgs& a) {
   if(a.M <= 8) {
     const dim3 grid((a.N + FEW_COLS - 1) / FEW_COLS), block(256);
@@ -249,12 +409,7 @@ template <typename T, int V> cudaError_t matmulLaunch(cudaStream_t st, const Mat
     if(a.M <= 4) return launchDependent(matmulFewKernel<T, 4, V>, grid, block, 0, st, a);
     return launchDependent(matmulFewKernel<T, 8, V>, grid, block, 0, st, a);
   }
-  constexpr int VT = V > 4 ? 4 : V;  // elements of the tile kernel's accesses: four threads per staged row
-  auto tiles = [&](int bm, int bn) { return ((long long)a.M + bm - 1) / bm * ((a.N + bn - 1) / bn); };
-  const int sms = smCount();
-  if(tiles(128, 128) >= 2 * sms) return launchDependent(matmulTileKernel<T, 128, 128, VT>, dim3((unsigned)tiles(128, 128)), dim3(256), 0, st, a);
-  if(tiles(64, 64) >= sms) return launchDependent(matmulTileKernel<T, 64, 64, VT>, dim3((unsigned)tiles(64, 64)), dim3(256), 0, st, a);
-  return launchDependent(matmulTileKernel<T, 32, 32, VT>, dim3((unsigned)tiles(32, 32)), dim3(256), 0, st, a);
+  return TileForms<T, V>::launch(st, a);
 }
 
 template <typename T> cudaError_t matmulLaunchT(cudaStream_t st, const MatmulArgs& a) {

@@ -2,8 +2,8 @@
 // and alignment, and the kernel that joins the parts of rows whose keys were cut over several blocks.
 //
 // The rows of a key head are its query heads' rows side by side: row r = token r / G, head kvHead * G + r % G with G = heads /
-// kvHeads, so that grouped heads read K and V once.  A block takes 64 such rows and a range of keys, 64 at a time: scores into
-// registers (4 x 4 per thread), a running maximum and sum per row, probabilities through shared memory, output accumulators in
+// kvHeads, so that grouped heads read K and V once.  A block takes 64 such rows (16 where there are no more) and a range of keys, 64 at a time: scores into
+// registers (4 x 4 or 1 x 4 per thread), a running maximum and sum per row, probabilities through shared memory, output accumulators in
 // registers.  All in fp32.  Keys behind a sequence's length are not read; masked keys' rows of K and V are replaced by zeros
 // while they are staged, so that nothing in them (NaN, Inf) reaches a product.
 //
@@ -20,24 +20,64 @@ namespace kb {
 
 namespace {
 
-constexpr int XS_ROWS = 64, XS_KEYS = 64, XS_THREADS = 256;
+constexpr int XS_KEYS = 64, XS_THREADS = 256;
 
 __host__ __device__ constexpr int xsPitch(int d) { return (d + 3) / 4 * 4 + 4; }
-size_t xsSmem(int dq, int dv) { return sizeof(float) * (size_t)((XS_ROWS + XS_KEYS) * xsPitch(dq) + XS_KEYS * xsPitch(dv) + XS_ROWS * (XS_KEYS + 4)) + XS_KEYS; }
+size_t xsSmem(int rows, int dq, int dv) { return sizeof(float) * (size_t)((rows + XS_KEYS) * xsPitch(dq) + XS_KEYS * xsPitch(dv) + rows * (XS_KEYS + 4)) + XS_KEYS; }
 
-// NC: groups of 64 output channels
-template <typename T, int NC>
+// Copies ROWS rows of d channels to fp32 rows of `pitch` in shared memory, zeros behind the last channel and for rows that
+// `row` gives no address for.  Eight lanes per row and four channels per lane, with several rows' loads in flight.
+template <typename T, int ROWS, bool VEC, class Row> __device__ __forceinline__ void xsStage(float* dst, int pitch, int d, Row row) {
+  constexpr int PASSES = (ROWS + XS_THREADS / 8 - 1) / (XS_THREADS / 8);
+  const int lane8 = threadIdx.x & 7, first = threadIdx.x >> 3;
+  const T* from[PASSES];
+#pragma unroll
+  for(int p = 0; p < PASSES; p++) {
+    const int r = first + p * (XS_THREADS / 8);
+    from[p] = r < ROWS ? row(r) : nullptr;
+  }
+  for(int c = lane8 * 4; c < pitch - 4; c += 32) {
+    float4 v[PASSES];
+#pragma unroll
+    for(int p = 0; p < PASSES; p++) {
+      v[p] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if(!from[p]) continue;
+      if(VEC) {  // d is a multiple of 4
+        OpVec<T, 4> w;
+        w.load(from[p] + c);
+        v[p] = make_float4(OpType<T>::to(w.e[0]), OpType<T>::to(w.e[1]), OpType<T>::to(w.e[2]), OpType<T>::to(w.e[3]));
+      }
+      else {
+        if(c < d) v[p].x = OpType<T>::to(from[p][c]);
+        if(c + 1 < d) v[p].y = OpType<T>::to(from[p][c + 1]);
+        if(c + 2 < d) v[p].z = OpType<T>::to(from[p][c + 2]);
+        if(c + 3 < d) v[p].w = OpType<T>::to(from[p][c + 3]);
+      }
+    }
+#pragma unroll
+    for(int p = 0; p < PASSES; p++) {
+      const int r = first + p * (XS_THREADS / 8);
+      if(r < ROWS) *reinterpret_cast<float4*>(dst + r * pitch + c) = v[p];
+    }
+  }
+}
+
+// NC: groups of 64 output channels; RI: rows per thread (16 threads share a row); VEC: channels in vectors of four
+template <typename T, int NC, int RI, bool VEC>
 __global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAttnArgs a, const XaSplit sp) {
   extern __shared__ float4 smem4[];
+  constexpr int ROWS = 16 * RI;
   const int pq = xsPitch(a.dq), pv = xsPitch(a.dv);
   constexpr int PP = XS_KEYS + 4;
   float* sQ = reinterpret_cast<float*>(smem4);
-  float* sK = sQ + XS_ROWS * pq;
+  float* sK = sQ + ROWS * pq;
   float* sV = sK + XS_KEYS * pq;
   float* sP = sV + XS_KEYS * pv;
-  uint8_t* sOk = reinterpret_cast<uint8_t*>(sP + XS_ROWS * PP);
+  uint8_t* sOk = reinterpret_cast<uint8_t*>(sP + ROWS * PP);
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const XaBlock blk = xaBlock(a, sp, XS_ROWS);
+  const int CG = NC > 1 || a.dv > 32 ? 16 : (a.dv > 16 ? 8 : (a.dv > 8 ? 4 : 2)), KS = 16 / CG;
+  const int cg = tx & (CG - 1), ks = tx / CG;
+  const XaBlock blk = xaBlock(a, sp, ROWS);
   const int G = a.heads / a.kvHeads;
   gridDepLaunch();
   gridDepWait();
@@ -46,16 +86,15 @@ __global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAtt
   const int keys = xaKeys(a, blk.b);
   const int k0 = blk.part * sp.chunk, k1 = (int)min((long long)keys, (long long)k0 + sp.chunk);
   if(sp.parts > 1 && k0 >= keys && blk.part > 0) return;  // a part without keys; part 0 always reports
-  auto rowQ = [&](int r) { return (const T*)a.q + blk.b * a.qB + (r / G) * a.qT + (blk.kvh * G + r % G) * a.qH; };
 
-  for(int i = tid; i < XS_ROWS * pq; i += XS_THREADS) {
-    const int r = i / pq, d = i - r * pq;
-    sQ[i] = (d < a.dq && blk.row0 + r < rows) ? OpType<T>::to(rowQ(blk.row0 + r)[d]) : 0.0f;
-  }
-  float mx[4], sum[4];
-  float4 o[4][NC];
+  xsStage<T, ROWS, VEC>(sQ, pq, a.dq, [&](int r) -> const T* {
+    r += blk.row0;
+    return r < rows ? (const T*)a.q + blk.b * a.qB + (r / G) * a.qT + (blk.kvh * G + r % G) * a.qH : nullptr;
+  });
+  float mx[RI], sum[RI];
+  float4 o[RI][NC];
 #pragma unroll
-  for(int i = 0; i < 4; i++) {
+  for(int i = 0; i < RI; i++) {
     mx[i] = -INFINITY;
     sum[i] = 0.0f;
 #pragma unroll
@@ -68,38 +107,37 @@ __global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAtt
     __syncthreads();
     if(tid < XS_KEYS) sOk[tid] = kt + tid < k1 && (!a.keyMask || a.keyMask[(int64_t)blk.b * a.kLen + kt + tid] != 0.0f);
     __syncthreads();
-    for(int i = tid; i < XS_KEYS * pq; i += XS_THREADS) {
-      const int j = i / pq, d = i - j * pq;
-      sK[i] = (d < a.dq && sOk[j]) ? OpType<T>::to(kBase[(kt + j) * a.kT + d]) : 0.0f;
-    }
-    for(int i = tid; i < XS_KEYS * pv; i += XS_THREADS) {
-      const int j = i / pv, d = i - j * pv;
-      sV[i] = (d < a.dv && sOk[j]) ? OpType<T>::to(vBase[(kt + j) * a.vT + d]) : 0.0f;
-    }
+    xsStage<T, XS_KEYS, VEC>(sK, pq, a.dq, [&](int j) { return sOk[j] ? kBase + (kt + j) * a.kT : nullptr; });
+    xsStage<T, XS_KEYS, VEC>(sV, pv, a.dv, [&](int j) { return sOk[j] ? vBase + (kt + j) * a.vT : nullptr; });
     __syncthreads();
-    float s[4][4];
+    // even and odd channels apart: the packed fp32 instructions do two IEEE operations per issue slot
+    float2 s2[RI][4];
 #pragma unroll
-    for(int i = 0; i < 4; i++)
+    for(int i = 0; i < RI; i++)
 #pragma unroll
-      for(int j = 0; j < 4; j++) s[i][j] = 0.0f;
-    for(int d = 0; d < a.dq; d += 4) {
-      float4 qv[4], kv[4];
+      for(int j = 0; j < 4; j++) s2[i][j] = make_float2(0.0f, 0.0f);
+#pragma unroll 4
+    for(int d = 0; d < pq - 4; d += 4) {
+      float4 qv[RI], kv[4];
 #pragma unroll
-      for(int i = 0; i < 4; i++) qv[i] = *reinterpret_cast<const float4*>(sQ + (ty * 4 + i) * pq + d);
+      for(int i = 0; i < RI; i++) qv[i] = *reinterpret_cast<const float4*>(sQ + (ty * RI + i) * pq + d);
 #pragma unroll
       for(int j = 0; j < 4; j++) kv[j] = *reinterpret_cast<const float4*>(sK + (tx + 16 * j) * pq + d);
 #pragma unroll
-      for(int i = 0; i < 4; i++)
+      for(int i = 0; i < RI; i++)
 #pragma unroll
         for(int j = 0; j < 4; j++) {
-          s[i][j] = fmaf(qv[i].x, kv[j].x, s[i][j]);
-          s[i][j] = fmaf(qv[i].y, kv[j].y, s[i][j]);
-          s[i][j] = fmaf(qv[i].z, kv[j].z, s[i][j]);
-          s[i][j] = fmaf(qv[i].w, kv[j].w, s[i][j]);
+          s2[i][j] = __ffma2_rn(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
+          s2[i][j] = __ffma2_rn(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
         }
     }
+    float s[RI][4];
 #pragma unroll
-    for(int i = 0; i < 4; i++) {
+    for(int i = 0; i < RI; i++)
+#pragma unroll
+      for(int j = 0; j < 4; j++) s[i][j] = s2[i][j].x + s2[i][j].y;
+#pragma unroll
+    for(int i = 0; i < RI; i++) {
       float top = -INFINITY;
 #pragma unroll
       for(int j = 0; j < 4; j++) {
@@ -117,38 +155,54 @@ __global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAtt
       for(int j = 0; j < 4; j++) {
         const float p = exp2f(s[i][j] - ref);
         part += p;
-        sP[(ty * 4 + i) * PP + tx + 16 * j] = p;
+        sP[(ty * RI + i) * PP + tx + 16 * j] = p;
       }
       sum[i] = sum[i] * keep + part;  // this thread's share of the row
 #pragma unroll
       for(int c = 0; c < NC; c++) { o[i][c].x *= keep; o[i][c].y *= keep; o[i][c].z *= keep; o[i][c].w *= keep; }
     }
     __syncthreads();
-    for(int j = 0; j < XS_KEYS; j++) {
-      float p[4];
+    // Output channels: CG threads have four each (of every 64 where there are more); the other threads of a row share the keys.
+    for(int j = ks * 4; j < XS_KEYS; j += 4 * KS) {
+      float4 p[RI];
 #pragma unroll
-      for(int i = 0; i < 4; i++) p[i] = sP[(ty * 4 + i) * PP + j];
+      for(int i = 0; i < RI; i++) p[i] = *reinterpret_cast<const float4*>(sP + (ty * RI + i) * PP + j);
 #pragma unroll
       for(int c = 0; c < NC; c++) {
-        const int d = c * 64 + tx * 4;
+        const int d = c * 64 + cg * 4;
         if(d >= a.dv) break;
-        const float4 v = *reinterpret_cast<const float4*>(sV + j * pv + d);
+        float4 v[4];
 #pragma unroll
-        for(int i = 0; i < 4; i++) {
-          o[i][c].x = fmaf(p[i], v.x, o[i][c].x);
-          o[i][c].y = fmaf(p[i], v.y, o[i][c].y);
-          o[i][c].z = fmaf(p[i], v.z, o[i][c].z);
-          o[i][c].w = fmaf(p[i], v.w, o[i][c].w);
+        for(int e = 0; e < 4; e++) v[e] = *reinterpret_cast<const float4*>(sV + (j + e) * pv + d);
+#pragma unroll
+        for(int i = 0; i < RI; i++) {
+          const float pe[4] = {p[i].x, p[i].y, p[i].z, p[i].w};
+#pragma unroll
+          for(int e = 0; e < 4; e++) {
+            const float2 pp = make_float2(pe[e], pe[e]);
+            const float2 lo = __ffma2_rn(pp, make_float2(v[e].x, v[e].y), make_float2(o[i][c].x, o[i][c].y));
+            const float2 hi = __ffma2_rn(pp, make_float2(v[e].z, v[e].w), make_float2(o[i][c].z, o[i][c].w));
+            o[i][c] = make_float4(lo.x, lo.y, hi.x, hi.y);
+          }
         }
       }
     }
   }
+  if(KS > 1)
 #pragma unroll
-  for(int i = 0; i < 4; i++) {
+    for(int i = 0; i < RI; i++)
+      for(int w = CG; w < 16; w *= 2) {
+        o[i][0].x += __shfl_xor_sync(0xffffffffu, o[i][0].x, w);
+        o[i][0].y += __shfl_xor_sync(0xffffffffu, o[i][0].y, w);
+        o[i][0].z += __shfl_xor_sync(0xffffffffu, o[i][0].z, w);
+        o[i][0].w += __shfl_xor_sync(0xffffffffu, o[i][0].w, w);
+      }
+#pragma unroll
+  for(int i = 0; i < RI; i++) {
     float total = sum[i];
 #pragma unroll
     for(int w = 8; w > 0; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
-    const int r = blk.row0 + ty * 4 + i;
+    const int r = blk.row0 + ty * RI + i;
     if(r >= rows) continue;
     if(sp.parts > 1) {
       float* part = xaPart(a, sp, blk, r, G);
@@ -156,8 +210,8 @@ __global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAtt
       for(int c = 0; c < NC; c++)
 #pragma unroll
         for(int e = 0; e < 4; e++) {
-          const int d = c * 64 + tx * 4 + e;
-          if(d < a.dv) part[2 + d] = reinterpret_cast<const float*>(&o[i][c])[e];
+          const int d = c * 64 + cg * 4 + e;
+          if(d < a.dv && ks == 0) part[2 + d] = reinterpret_cast<const float*>(&o[i][c])[e];
         }
       if(tx == 0) { part[0] = mx[i]; part[1] = total; }
       continue;
@@ -169,8 +223,8 @@ __global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAtt
     for(int c = 0; c < NC; c++)
 #pragma unroll
       for(int e = 0; e < 4; e++) {
-        const int d = c * 64 + tx * 4 + e;
-        if(d < a.dv) out[d] = OpType<T>::from(live ? reinterpret_cast<const float*>(&o[i][c])[e] * inv : 0.0f);
+        const int d = c * 64 + cg * 4 + e;
+        if(d < a.dv && ks == 0) out[d] = OpType<T>::from(live ? reinterpret_cast<const float*>(&o[i][c])[e] * inv : 0.0f);
       }
   }
 }
@@ -219,16 +273,26 @@ __global__ void __launch_bounds__(256) crossAttnJoinKernel(const CrossAttnArgs a
   }
 }
 
-template <typename T, int NC> cudaError_t simtLaunch(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp) {
-  const cudaError_t e = allowSharedMemory((const void*)crossAttnSimtKernel<T, NC>, 227 * 1024);
+template <typename T, int NC, int RI, bool VEC> cudaError_t simtLaunch(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp) {
+  static SharedMemoryOptIn optIn;
+  const cudaError_t e = optIn((const void*)crossAttnSimtKernel<T, NC, RI, VEC>, 227 * 1024);
   if(e != cudaSuccess) return e;
-  return launchDependent(crossAttnSimtKernel<T, NC>, dim3(sp.blocks), dim3(XS_THREADS), xsSmem(a.dq, a.dv), st, a, sp);
+  return launchDependent(crossAttnSimtKernel<T, NC, RI, VEC>, dim3(sp.blocks), dim3(XS_THREADS), xsSmem(16 * RI, a.dq, a.dv), st, a, sp);
 }
-template <typename T> cudaError_t simtLaunchT(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp) {
-  if(a.dv <= 64) return simtLaunch<T, 1>(st, a, sp);
-  if(a.dv <= 128) return simtLaunch<T, 2>(st, a, sp);
-  return simtLaunch<T, 4>(st, a, sp);
+template <typename T, int NC> cudaError_t simtLaunchNC(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp, int rows) {
+  const uintptr_t p = (uintptr_t)a.q | (uintptr_t)a.k | (uintptr_t)a.v;
+  const int64_t strides = a.qB | a.qT | a.qH | a.kB | a.kT | a.kH | a.vB | a.vT | a.vH;
+  const bool vec = p % (4 * sizeof(T)) == 0 && strides % 4 == 0 && a.dq % 4 == 0 && a.dv % 4 == 0;
+  if(rows == 16) return vec ? simtLaunch<T, NC, 1, true>(st, a, sp) : simtLaunch<T, NC, 1, false>(st, a, sp);
+  return vec ? simtLaunch<T, NC, 4, true>(st, a, sp) : simtLaunch<T, NC, 4, false>(st, a, sp);
 }
+template <typename T> cudaError_t simtLaunchT(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp, int rows) {
+  if(a.dv <= 64) return simtLaunchNC<T, 1>(st, a, sp, rows);
+  if(a.dv <= 128) return simtLaunchNC<T, 2>(st, a, sp, rows);
+  return simtLaunchNC<T, 4>(st, a, sp, rows);
+}
+// Rows of a block of the CUDA-core kernel.
+int simtRows(int qLen, int heads, int kvHeads) { return (long long)qLen * (heads / kvHeads) <= 16 ? 16 : 64; }
 
 }  // namespace
 
@@ -276,7 +340,7 @@ Plan planFor(int dt, int batch, int qLen, int kLen, int heads, int kvHeads, int 
   Plan p = {};
   p.tc = crossAttnTcSizes(dt, heads, kvHeads, dq, dv);
   if(p.tc) p.sp = crossAttnTcSplit(batch, qLen, kLen, heads, kvHeads, dv, &p.tilesPerBlock);
-  else p.sp = xaPlanSplit(XS_ROWS, XS_KEYS, 2, batch, qLen, kLen, heads, kvHeads, dv);
+  else p.sp = xaPlanSplit(simtRows(qLen, heads, kvHeads), XS_KEYS, 2, batch, qLen, kLen, heads, kvHeads, dv);
   return p;
 }
 
@@ -292,16 +356,17 @@ cudaError_t launchCrossAttn(cudaStream_t st, const CrossAttnArgs& a) {
   XaSplit& sp = p.sp;
   if(p.tc && !crossAttnAligned(a)) {
     p.tc = false;
-    sp.rowTiles = (int)(((long long)a.qLen * (a.heads / a.kvHeads) + XS_ROWS - 1) / XS_ROWS);
+    const int rows = simtRows(a.qLen, a.heads, a.kvHeads);
+    sp.rowTiles = (int)(((long long)a.qLen * (a.heads / a.kvHeads) + rows - 1) / rows);
     sp.blocks = (unsigned)((long long)a.batch * a.kvHeads * sp.rowTiles * sp.parts);
   }
   cudaError_t e;
   if(p.tc) e = launchCrossAttnTc(st, a, sp, p.tilesPerBlock);
   else
     switch(a.dt) {
-      case DT_F32: e = simtLaunchT<float>(st, a, sp); break;
-      case DT_F16: e = simtLaunchT<__half>(st, a, sp); break;
-      default: e = simtLaunchT<__nv_bfloat16>(st, a, sp); break;
+      case DT_F32: e = simtLaunchT<float>(st, a, sp, simtRows(a.qLen, a.heads, a.kvHeads)); break;
+      case DT_F16: e = simtLaunchT<__half>(st, a, sp, simtRows(a.qLen, a.heads, a.kvHeads)); break;
+      default: e = simtLaunchT<__nv_bfloat16>(st, a, sp, simtRows(a.qLen, a.heads, a.kvHeads)); break;
     }
   if(e != cudaSuccess || sp.parts == 1) return e;
   const long long rows = (long long)a.batch * a.qLen * a.heads;
