@@ -64,7 +64,7 @@ template <typename T, int ROWS, bool VEC, class Row> __device__ __forceinline__ 
 
 // NC: groups of 64 output channels; RI: rows per thread (16 threads share a row); VEC: channels in vectors of four
 template <typename T, int NC, int RI, bool VEC>
-__global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAttnArgs a, const XaSplit sp) {
+__global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 ? 2 : 1)) : (NC <= 2 ? 2 : 1)) crossAttnSimtKernel(const CrossAttnArgs a, const XaSplit sp) {
   extern __shared__ float4 smem4[];
   constexpr int ROWS = 16 * RI;
   const int pq = xsPitch(a.dq), pv = xsPitch(a.dv);
@@ -229,48 +229,112 @@ __global__ void __launch_bounds__(XS_THREADS) crossAttnSimtKernel(const CrossAtt
   }
 }
 
-// One warp per row: the parts' states, added in the order of the keys.
+// One block per row: the parts' weights, then the parts' states, added in the order of the keys.  The threads beyond a row's channels
+// take another stretch of the parts.
+constexpr int XJ_THREADS = 256;
 template <typename T>
-__global__ void __launch_bounds__(256) crossAttnJoinKernel(const CrossAttnArgs a, const XaSplit sp) {
+__global__ void __launch_bounds__(XJ_THREADS) crossAttnJoinKernel(const CrossAttnArgs a, const XaSplit sp) {
+  __shared__ float sW[XA_MAX_PARTS], sTop[XJ_THREADS / 32], sO[XJ_THREADS], sTotal[XJ_THREADS / 32];
+  gridDepLaunch();
+  gridDepWait();
+  const int G = a.heads / a.kvHeads, tid = threadIdx.x;
+  const long long perHead = (long long)a.qLen * G, bh = blockIdx.x / perHead;
+  const int r = (int)(blockIdx.x - bh * perHead);
+  XaBlock blk;
+  blk.b = (int)(bh / a.kvHeads);
+  blk.kvh = (int)(bh - (long long)blk.b * a.kvHeads);
+  blk.row0 = 0;
+  blk.part = 0;
+  if(r >= xaRows(a, blk.b, G)) return;
+  const int parts = max(1, (int)(((long long)xaKeys(a, blk.b) + sp.chunk - 1) / sp.chunk));
+  const float* state = xaPart(a, sp, blk, r, G);
+  // weights
+  const float top0 = tid < parts ? state[(int64_t)tid * sp.pitch] : -INFINITY;
+  static_assert(XA_MAX_PARTS <= XJ_THREADS, "a thread per part");
+  float top = top0;
+#pragma unroll
+  for(int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  if((tid & 31) == 0) sTop[tid >> 5] = top;
+  __syncthreads();
+#pragma unroll
+  for(int w = 0; w < XJ_THREADS / 32; w++) top = fmaxf(top, sTop[w]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f;
+  if(tid < parts) {
+    const float w = exp2f(top0 - ref);
+    sW[tid] = w;
+    total = w * state[(int64_t)tid * sp.pitch + 1];
+  }
+#pragma unroll
+  for(int w = 16; w > 0; w >>= 1) total += __shfl_xor_sync(0xffffffffu, total, w);
+  if((tid & 31) == 0) sTotal[tid >> 5] = total;
+  __syncthreads();
+  total = 0.0f;
+#pragma unroll
+  for(int w = 0; w < XJ_THREADS / 32; w++) total += sTotal[w];
+  // channels
+  const int width = a.dv <= 32 ? 32 : (a.dv <= 64 ? 64 : (a.dv <= 128 ? 128 : 256)), shares = XJ_THREADS / width;
+  const int d = tid & (width - 1), share = tid / width;
+  float o = 0.0f;
+  if(d < a.dv) {
+    const int p1 = (share + 1) * parts / shares;
+#pragma unroll 8
+    for(int p = share * parts / shares; p < p1; p++) o = fmaf(sW[p], state[(int64_t)p * sp.pitch + 2 + d], o);
+  }
+  sO[tid] = o;
+  __syncthreads();
+  if(share > 0 || d >= a.dv) return;
+  for(int s = 1; s < shares; s++) o += sO[s * width + d];
+  const bool live = total != 0.0f && (!a.queryMask || a.queryMask[(int64_t)blk.b * a.qLen + r / G] != 0.0f);
+  T* out = (T*)a.out + blk.b * a.oB + (r / G) * a.oT + (blk.kvh * G + r % G) * a.oH;
+  out[d] = OpType<T>::from(live ? o * (1.0f / total) : 0.0f);
+}
+
+// The same with a warp per row, for many rows (which have few parts): 34 656 rows of two parts took 110 us with a block each.
+template <typename T>
+__global__ void __launch_bounds__(XJ_THREADS) crossAttnJoinManyKernel(const CrossAttnArgs a, const XaSplit sp) {
   gridDepLaunch();
   gridDepWait();
   const int G = a.heads / a.kvHeads, lane = threadIdx.x & 31;
-  const long long all = (long long)a.batch * a.kvHeads * a.qLen * G;
-  for(long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < all; i += (long long)gridDim.x * 8) {
-    const long long perHead = (long long)a.qLen * G;
-    XaBlock blk;
-    const long long bh = i / perHead;
-    const int r = (int)(i - bh * perHead);
-    blk.b = (int)(bh / a.kvHeads);
-    blk.kvh = (int)(bh - (long long)blk.b * a.kvHeads);
-    blk.row0 = 0;
-    if(r >= xaRows(a, blk.b, G)) continue;
-    const int keys = xaKeys(a, blk.b);
-    const int parts = max(1, (int)(((long long)keys + sp.chunk - 1) / sp.chunk));
-    float top = -INFINITY;
-    for(int p = lane; p < parts; p += 32) { blk.part = p; top = fmaxf(top, xaPart(a, sp, blk, r, G)[0]); }
+  const long long perHead = (long long)a.qLen * G, i = (long long)blockIdx.x * (XJ_THREADS / 32) + (threadIdx.x >> 5), bh = i / perHead;
+  if(bh >= (long long)a.batch * a.kvHeads) return;
+  const int r = (int)(i - bh * perHead);
+  XaBlock blk;
+  blk.b = (int)(bh / a.kvHeads);
+  blk.kvh = (int)(bh - (long long)blk.b * a.kvHeads);
+  blk.row0 = 0;
+  blk.part = 0;
+  if(r >= xaRows(a, blk.b, G)) return;
+  const int parts = max(1, (int)(((long long)xaKeys(a, blk.b) + sp.chunk - 1) / sp.chunk));
+  const float* state = xaPart(a, sp, blk, r, G);
+  float top = -INFINITY;
+  for(int p = lane; p < parts; p += 32) top = fmaxf(top, state[(int64_t)p * sp.pitch]);
 #pragma unroll
-    for(int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f, o[8];
+  for(int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f, o[8];
 #pragma unroll
-    for(int c = 0; c < 8; c++) o[c] = 0.0f;
-    for(int p = 0; p < parts; p++) {
-      blk.part = p;
-      const float* part = xaPart(a, sp, blk, r, G);
-      const float w = exp2f(part[0] - ref);
-      total += w * part[1];
-#pragma unroll
-      for(int c = 0; c < 8; c++)
-        if(c * 32 + lane < a.dv) o[c] = fmaf(w, part[2 + c * 32 + lane], o[c]);
-    }
-    const bool live = total != 0.0f && (!a.queryMask || a.queryMask[(int64_t)blk.b * a.qLen + r / G] != 0.0f);
-    const float inv = 1.0f / total;
-    T* out = (T*)a.out + blk.b * a.oB + (r / G) * a.oT + (blk.kvh * G + r % G) * a.oH;
+  for(int c = 0; c < 8; c++) o[c] = 0.0f;
+#pragma unroll 2
+  for(int p = 0; p < parts; p++) {
+    const float* part = state + (int64_t)p * sp.pitch;
+    const float w = exp2f(part[0] - ref);
+    total += w * part[1];
 #pragma unroll
     for(int c = 0; c < 8; c++)
-      if(c * 32 + lane < a.dv) out[c * 32 + lane] = OpType<T>::from(live ? o[c] * inv : 0.0f);
+      if(c * 32 + lane < a.dv) o[c] = fmaf(w, part[2 + c * 32 + lane], o[c]);
   }
+  const bool live = total != 0.0f && (!a.queryMask || a.queryMask[(int64_t)blk.b * a.qLen + r / G] != 0.0f);
+  const float inv = 1.0f / total;
+  T* out = (T*)a.out + blk.b * a.oB + (r / G) * a.oT + (blk.kvh * G + r % G) * a.oH;
+#pragma unroll
+  for(int c = 0; c < 8; c++)
+    if(c * 32 + lane < a.dv) out[c * 32 + lane] = OpType<T>::from(live ? o[c] * inv : 0.0f);
+}
+template <typename T> cudaError_t joinLaunch(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp) {
+  const long long rows = (long long)a.batch * a.qLen * a.heads;
+  if(rows < 8LL * smCount()) return launchDependent(crossAttnJoinKernel<T>, dim3((unsigned)rows), dim3(XJ_THREADS), 0, st, a, sp);
+  return launchDependent(crossAttnJoinManyKernel<T>, dim3((unsigned)((rows + XJ_THREADS / 32 - 1) / (XJ_THREADS / 32))), dim3(XJ_THREADS), 0, st, a, sp);
 }
 
 template <typename T, int NC, int RI, bool VEC> cudaError_t simtLaunch(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp) {
@@ -296,17 +360,17 @@ int simtRows(int qLen, int heads, int kvHeads) { return (long long)qLen * (heads
 
 }  // namespace
 
-XaSplit xaPlanSplit(int rowsPerBlock, int keysPerStep, int blocksPerSm, int batch, int qLen, int kLen, int heads, int kvHeads, int dv) {
+XaSplit xaPlanSplit(int rowsPerBlock, int keysPerStep, int keysWorthABlock, int blocksPerSm, int batch, int qLen, int kLen, int heads, int kvHeads, int dv) {
   XaSplit sp;
   const long long rows = (long long)qLen * (heads / kvHeads);
   sp.rowTiles = (int)((rows + rowsPerBlock - 1) / rowsPerBlock);
-  const long long whole = (long long)batch * kvHeads * sp.rowTiles;
-  // Keys are cut where the uncut blocks would leave most of the GPU idle, into as many parts as fill it about twice, of at
-  // least two steps.
-  const long long room = (long long)blocksPerSm * smCount();
-  long long parts = 1;
-  if(whole * 2 <= room) parts = std::min<long long>(2 * room / whole, ((long long)kLen + 2 * keysPerStep - 1) / (2 * keysPerStep));
-  if(parts < 1) parts = 1;
+  const long long whole = (long long)batch * kvHeads * sp.rowTiles, room = (long long)blocksPerSm * smCount();
+  // Parts of the keys.  So many that the blocks fill the GPU once, of at least two steps; and up to four times as many where their
+  // parts stay long against what a block costs besides: sequences of different lengths, and the end of the last round, are then
+  // shared out evenly (8 sequences of 0 to 32768 keys, 8 key heads of 128, bf16: 109 us in 4 parts of 8192).
+  const long long once = std::min<long long>(room / whole, kLen / (2LL * keysPerStep));
+  const long long even = std::min<long long>(4 * room / whole, kLen / keysWorthABlock);
+  const long long parts = std::min<long long>(XA_MAX_PARTS, std::max<long long>(1, std::max(once, even)));
   long long chunk = ((long long)kLen + parts - 1) / parts;
   chunk = std::max<long long>(keysPerStep, (chunk + keysPerStep - 1) / keysPerStep * keysPerStep);
   sp.chunk = (int)std::min<long long>(chunk, 1LL << 30);
@@ -332,15 +396,19 @@ bool crossAttnAligned(const CrossAttnArgs& a) {
 // What a call runs.  The workspace is a function of the sizes alone, so the plan is too: where the sizes suit the tensor cores and
 // only the tensors' alignment does not, the CUDA-core kernel cuts the keys as the other would.
 struct Plan {
-  bool tc;
+  enum { SIMT, FEW, TC } kind;
   int tilesPerBlock;
   XaSplit sp;
 };
 Plan planFor(int dt, int batch, int qLen, int kLen, int heads, int kvHeads, int dq, int dv) {
   Plan p = {};
-  p.tc = crossAttnTcSizes(dt, heads, kvHeads, dq, dv);
-  if(p.tc) p.sp = crossAttnTcSplit(batch, qLen, kLen, heads, kvHeads, dv, &p.tilesPerBlock);
-  else p.sp = xaPlanSplit(simtRows(qLen, heads, kvHeads), XS_KEYS, 2, batch, qLen, kLen, heads, kvHeads, dv);
+  p.kind = !crossAttnTcSizes(dt, heads, kvHeads, dq, dv) ? Plan::SIMT : ((long long)qLen * (heads / kvHeads) <= 16 ? Plan::FEW : Plan::TC);
+  if(p.kind == Plan::TC) p.sp = crossAttnTcSplit(batch, qLen, kLen, heads, kvHeads, dv, &p.tilesPerBlock);
+  else if(p.kind == Plan::FEW) p.sp = crossAttnFewSplit(batch, qLen, kLen, heads, kvHeads, dq, dv);
+  else {
+    const int rows = simtRows(qLen, heads, kvHeads);
+    p.sp = xaPlanSplit(rows, XS_KEYS, 512, rows == 16 && dq <= 64 && dv <= 64 ? 4 : 2, batch, qLen, kLen, heads, kvHeads, dv);
+  }
   return p;
 }
 
@@ -354,14 +422,15 @@ cudaError_t launchCrossAttn(cudaStream_t st, const CrossAttnArgs& a) {
   if(a.batch == 0 || a.qLen == 0) return cudaSuccess;
   Plan p = planFor(a.dt, a.batch, a.qLen, a.kLen, a.heads, a.kvHeads, a.dq, a.dv);
   XaSplit& sp = p.sp;
-  if(p.tc && !crossAttnAligned(a)) {
-    p.tc = false;
+  if(p.kind != Plan::SIMT && !crossAttnAligned(a)) {
+    p.kind = Plan::SIMT;
     const int rows = simtRows(a.qLen, a.heads, a.kvHeads);
     sp.rowTiles = (int)(((long long)a.qLen * (a.heads / a.kvHeads) + rows - 1) / rows);
     sp.blocks = (unsigned)((long long)a.batch * a.kvHeads * sp.rowTiles * sp.parts);
   }
   cudaError_t e;
-  if(p.tc) e = launchCrossAttnTc(st, a, sp, p.tilesPerBlock);
+  if(p.kind == Plan::TC) e = launchCrossAttnTc(st, a, sp, p.tilesPerBlock);
+  else if(p.kind == Plan::FEW) e = launchCrossAttnFew(st, a, sp);
   else
     switch(a.dt) {
       case DT_F32: e = simtLaunchT<float>(st, a, sp, simtRows(a.qLen, a.heads, a.kvHeads)); break;
@@ -369,12 +438,10 @@ cudaError_t launchCrossAttn(cudaStream_t st, const CrossAttnArgs& a) {
       default: e = simtLaunchT<__nv_bfloat16>(st, a, sp, simtRows(a.qLen, a.heads, a.kvHeads)); break;
     }
   if(e != cudaSuccess || sp.parts == 1) return e;
-  const long long rows = (long long)a.batch * a.qLen * a.heads;
-  const dim3 grid((unsigned)std::min<long long>((rows + 7) / 8, 16LL * smCount()));
   switch(a.dt) {
-    case DT_F32: return launchDependent(crossAttnJoinKernel<float>, grid, dim3(256), 0, st, a, sp);
-    case DT_F16: return launchDependent(crossAttnJoinKernel<__half>, grid, dim3(256), 0, st, a, sp);
-    default: return launchDependent(crossAttnJoinKernel<__nv_bfloat16>, grid, dim3(256), 0, st, a, sp);
+    case DT_F32: return joinLaunch<float>(st, a, sp);
+    case DT_F16: return joinLaunch<__half>(st, a, sp);
+    default: return joinLaunch<__nv_bfloat16>(st, a, sp);
   }
 }
 

@@ -17,13 +17,18 @@ struct XaSplit {
   int pitch;      // floats of a part's state: maximum, sum, unnormalised output
   size_t workspace;
 };
-// Cuts the keys of blocks of rowsPerBlock rows where the uncut blocks would leave most of the GPU idle.
-XaSplit xaPlanSplit(int rowsPerBlock, int keysPerStep, int blocksPerSm, int batch, int qLen, int kLen, int heads, int kvHeads, int dv);
+constexpr int XA_MAX_PARTS = 256;
+// Cuts the keys of blocks of rowsPerBlock rows where the uncut blocks would leave part of the GPU idle.
+XaSplit xaPlanSplit(int rowsPerBlock, int keysPerStep, int keysWorthABlock, int blocksPerSm, int batch, int qLen, int kLen, int heads, int kvHeads, int dv);
 
 // kb_xattn_tc.cu: sizes that the tensor-core kernel takes (and rows on 16-byte boundaries)
 bool crossAttnTcSizes(int dt, int heads, int kvHeads, int dq, int dv);
 XaSplit crossAttnTcSplit(int batch, int qLen, int kLen, int heads, int kvHeads, int dv, int* tilesPerBlock);
 cudaError_t launchCrossAttnTc(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp, int tilesPerBlock);
+
+// kb_xattn_few.cu: the same sizes, up to 16 rows of a key head
+XaSplit crossAttnFewSplit(int batch, int qLen, int kLen, int heads, int kvHeads, int dq, int dv);
+cudaError_t launchCrossAttnFew(cudaStream_t st, const CrossAttnArgs& a, const XaSplit& sp);
 
 struct XaBlock {
   int b, kvh, row0, part;

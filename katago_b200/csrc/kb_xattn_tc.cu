@@ -514,7 +514,7 @@ XaSplit crossAttnTcSplit(int batch, int qLen, int kLen, int heads, int kvHeads, 
   const int G = heads / kvHeads, tileRows = 128 / G * G;
   const long long rows = (long long)qLen * G, pairs = (rows + 2 * tileRows - 1) / (2 * tileRows) * batch * kvHeads;
   *tilesPerBlock = rows > tileRows && pairs >= smCount() ? 2 : 1;
-  return xaPlanSplit(tileRows * *tilesPerBlock, XT_KEYS, 1, batch, qLen, kLen, heads, kvHeads, dv);
+  return xaPlanSplit(tileRows * *tilesPerBlock, XT_KEYS, 1024, 1, batch, qLen, kLen, heads, kvHeads, dv);
 }
 
 cudaError_t launchCrossAttnTc(cudaStream_t st, const CrossAttnArgs& x, const XaSplit& sp, int tilesPerBlock) {
