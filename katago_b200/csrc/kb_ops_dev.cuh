@@ -47,13 +47,16 @@ template <typename T> __device__ __forceinline__ float opAct(float v, int act) {
 // Bounded wait of a role of these kernels (about 2 s).  A wait that runs out raises the abort flag and leaves `code` in the status
 // word, which is page-locked host memory (hence a plain store); it returns false, as does one that finds the flag raised, and
 // the role then leaves its loops.
-static __device__ __noinline__ bool opWaitOn(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
-  const uint64_t t0 = globalTimerNs();
+// The clock is read only after some dozens of tries: reading it takes longer than most waits do.
+__device__ __forceinline__ bool opWaitSpin(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
+  uint64_t t0 = 0;
   for(uint32_t spins = 1;; spins++) {
     if(mbarTryWait(bar, parity)) return true;
     if((spins & 63u) == 0u) {
       if(*abortFlag) return false;
-      if(globalTimerNs() - t0 > 2000000000ull) {
+      const uint64_t now = globalTimerNs();
+      if(t0 == 0) t0 = now;
+      else if(now - t0 > 2000000000ull) {
         *abortFlag = 1;
         *status = code;
         __threadfence_system();
@@ -62,8 +65,15 @@ static __device__ __noinline__ bool opWaitOn(uint32_t bar, uint32_t parity, vola
     }
   }
 }
+static __device__ __noinline__ bool opWaitOn(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
+  return opWaitSpin(bar, parity, abortFlag, status, code);
+}
 __device__ __forceinline__ bool opWait(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
   return mbarTryWait(bar, parity) != 0u || opWaitOn(bar, parity, abortFlag, status, code);
+}
+// The same in line, for kernels that move registers between warpgroups (ptxas finds no allocation with a call in them).
+__device__ __forceinline__ bool opWaitInline(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
+  return opWaitSpin(bar, parity, abortFlag, status, code);
 }
 
 __device__ __forceinline__ void tmaLoad4d(uint32_t dst, const CUtensorMap* tmap, int c0, int c1, int c2, int c3, uint32_t bar) {
@@ -80,17 +90,6 @@ __device__ __forceinline__ void tmemLd16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 __device__ __forceinline__ void tmemLdWaitFor(uint32_t (&r)[16]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]) : : "memory");
-}
-
-// The same in line, for kernels that move registers between warpgroups (ptxas finds no allocation with a call in them).
-__device__ __forceinline__ bool opWaitInline(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
-  if(mbarWait(bar, parity, abortFlag)) return true;
-  if(*abortFlag == 0) {
-    *abortFlag = 1;
-    *status = code;
-    __threadfence_system();
-  }
-  return false;
 }
 
 // Two values in one 32-bit word of the 16-bit type, the first in the low half.

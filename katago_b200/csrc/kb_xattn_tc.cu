@@ -21,11 +21,17 @@
 // (With a test of a bit per score in both passes: 341 us for 64 x 6 heads of 361 tokens over up to 2888 states, a fifth masked.)
 // Rows of the tile that are no tokens are computed and not written.
 //
-// What bounds it: the exponentials.  The special-function units give 16 per clock and SM, 1024 cycles for 128 x 128, as long as the
-// two products of head size 128 take and twice as long as those of 64.  So a share of them (XtShape::POLY pairs of every eight) is
-// computed on the FMA units: t = n + f with n whole and |f| <= 1/2, 2^f by a polynomial, n added to the exponent's bits.  The
-// polynomials are minimax fits of the relative error over [-1/2, 1/2] (Remez exchange): degree 3 is off by 7.5e-5 at most, for
-// bf16 probabilities, whose rounding is 3.9e-3; degree 4 by 2.6e-6, for fp16 with 4.9e-4.
+// What bounds it: the softmax of a row tile, some 700 instructions of a warp per 128 keys with two warps to a scheduler, beside the MMAs
+// (1024 cycles for the two products of 128 x 128 with head size 128, half of it with 64).  A step of both row tiles takes 3000
+// cycles with head size 64 and 3200 with 128; the special-function units (16 exponentials per clock and SM, 2048 cycles) are the
+// busiest part.  So one pair of exponentials in eight is computed on the FMA units (t = n + f with n whole and |f| <= 1/2, 2^f by a
+// polynomial, n added to the exponent's bits): 2 x 4096 x 8192 tokens, 16 heads of 128, bf16: 520 us with none, 493 with one, 511 with
+// two, 540 with three.  The polynomials are minimax fits of the relative error over [-1/2, 1/2] (Remez exchange): degree 3 is off by
+// 7.5e-5 at most, for bf16 probabilities, whose rounding is 3.9e-3; degree 4 by 2.6e-6, for fp16 with 4.9e-4.
+// What did not help: four threads' warps to a scheduler (a row by two threads, 70 us where this takes 57); an issuing warp per row tile.
+//
+// Blocks of the longest sequences come first, where the batch is ragged: else the last ones started may be the longest (64 x 6 heads of
+// 361 tokens over up to 2888 states, fp16: 147 us, 160 us in the order of the batch).
 #include "kb_kernels.cuh"
 #include "kb_ops.h"
 #include "kb_ops_dev.cuh"
@@ -41,11 +47,12 @@ constexpr int XT_THREADS = 384, XT_KEYS = 128, XT_ERR = 311;
 constexpr int XT_HALF = 128 * 64 * 2;  // bytes of 128 rows x 64 channels
 constexpr float XT_GROW = 8.0f;
 enum { XT_ALL, XT_SOME, XT_NONE };
+constexpr int XT_SORT = 128;  // sequences that a block ranks
 
 struct CrossAttnTcArgs {
   CrossAttnArgs x;
   XaSplit sp;
-  int G, tileTokens, tileRows, tilesPerBlock;
+  int G, tileTokens, tileRows, tilesPerBlock, longestFirst;
   int qUse[3], kUse[3], vUse[3];  // 0 where a tensor repeats along the batch / token / head dimension
 };
 
@@ -54,7 +61,6 @@ template <int D> struct XtShape {
   static constexpr int HALVES = D / 64;
   static constexpr int TILE = HALVES * XT_HALF;          // bytes of 128 rows
   static constexpr int STAGES = D == 64 ? 4 : 2;         // tiles of K, and of V, in flight
-  static constexpr int POLY = D == 64 ? 3 : 2;
   static constexpr bool APART = D == 64;                 // probabilities have columns of their own
   static constexpr uint32_t O_AT = 256, P_AT = APART ? 256 + 2 * D : 0, P_STEP = APART ? 64 : 128;
   static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + STAGES * XT_KEYS * 4 + 4 * 128 * 4 + 1024 + 512;
@@ -66,17 +72,28 @@ __device__ __forceinline__ float max3Nan(float a, float b, float c) {
   return d;
 }
 
-// 2^t of two numbers up to some 100 on the FMA units; below -126 as for -126.  A NaN does not survive it: rows that have one get
-// a reference of NaN, which the exponentials of the special-function units carry on.
-template <typename T> __device__ __forceinline__ float2 ex2Poly(float2 t) {
+// 64 columns of this thread's row, complete: load and wait in one statement, whose results are outputs only (naming the registers of
+// an earlier load as in and out of the wait costs a copy of each).
+__device__ __forceinline__ void tmemLd64Now(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+    "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%64];\n\ttcgen05.wait::ld.sync.aligned;"
+    : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]) : "r"(taddr) : "memory");
+}
+
+// 2^t of two numbers t = 142 u - 126 up to 16 (twice what a maximum may lag), u cut to [0, 1]: below t = -126 as for -126.  A NaN does not survive it: rows that have one get a reference of NaN, which the exponentials of the special-function
+// units carry on.
+__device__ __forceinline__ float fmaSat(float a, float b, float c) {
+  float d;
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <typename T> __device__ __forceinline__ float2 ex2Poly(float2 u) {
   constexpr bool LONG = std::is_same<T, __half>::value;
-  t.x = fmaxf(t.x, -126.0f);
-  t.y = fmaxf(t.y, -126.0f);
-  const float2 magic = make_float2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's low bits are the nearest whole number
-  const float2 r = __fadd2_rn(t, magic);
-  const float2 n = __fadd2_rn(r, make_float2(-12582912.0f, -12582912.0f));
-  const float2 f = __ffma2_rn(n, make_float2(-1.0f, -1.0f), t);
   auto both = [](float c) { return make_float2(c, c); };
+  // 1.5 * 2^23: the sum's low bits are the nearest whole number
+  const float2 r = __ffma2_rn(u, both(142.0f), both(12582912.0f - 126.0f));
+  const float2 n = __fadd2_rn(r, both(-(12582912.0f - 126.0f)));
+  const float2 f = __ffma2_rn(u, both(142.0f), make_float2(-n.x, -n.y));
   float2 p;
   if(LONG) {
     p = __ffma2_rn(f, both(0.009570102207362652f), both(0.05591785907745361f));
@@ -120,6 +137,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
   int* sKind = reinterpret_cast<int*>(sState + 4 * 128);  // [ST] XT_ALL, XT_SOME or XT_NONE of a tile's keys are attended
   uint32_t* tmemSlot = reinterpret_cast<uint32_t*>(sKind + ST);
   volatile int* abortFlag = reinterpret_cast<volatile int*>(tmemSlot + 1);
+  volatile int* sSeq = abortFlag + 1;                 // this block's sequence, where the sequences are ranked
 
   const CrossAttnArgs& x = a.x;
   const int warp = warpIndex(), lane = threadIdx.x & 31;
@@ -135,12 +153,28 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
   }
   if(warp == 9) { tmemAlloc(smemU32(tmemSlot), 512); tmemRelinquish(); }
   tcFenceBefore();
+  if(warp == 8 && electOne()) { prefetchTensorMap(&tmQ); prefetchTensorMap(&tmK); prefetchTensorMap(&tmV); }
   __syncthreads();
   tcFenceAfter();
   gridDepLaunch();
   gridDepWait();
   const uint32_t tmem = *tmemSlot;
-  const XaBlock blk = xaBlock(x, a.sp, a.tileRows * a.tilesPerBlock);
+  XaBlock blk = xaBlock(x, a.sp, a.tileRows * a.tilesPerBlock);
+  if(a.longestFirst) {
+    // the sequence of this block's rank by length (ties by number): a thread counts for each how many come before it
+    int* sLen = reinterpret_cast<int*>(sState);
+    const int i = threadIdx.x;
+    if(i < x.batch) sLen[i] = xaKeys(x, i);
+    __syncthreads();
+    if(i < x.batch) {
+      const int mine = sLen[i];
+      int before = 0;
+      for(int j = 0; j < x.batch; j++) before += sLen[j] > mine || (sLen[j] == mine && j < i) ? 1 : 0;
+      if(before == blk.b) *sSeq = i;
+    }
+    __syncthreads();
+    blk.b = *sSeq;
+  }
   const int rows = xaRows(x, blk.b, a.G), keys = xaKeys(x, blk.b);
   const int k0 = blk.part * a.sp.chunk, k1 = (int)min((long long)keys, (long long)k0 + a.sp.chunk);
   const bool idle = blk.row0 >= rows || (blk.part > 0 && k0 >= keys);  // part 0 reports a row without keys
@@ -153,7 +187,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
   auto wait = [&](uint64_t* bar, uint32_t parity) { return opWaitInline(smemU32(bar), parity, abortFlag, x.status, XT_ERR); };
 
   if(warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     const int qHalves = (x.dq + 63) / 64, vHalves = (x.dv + 63) / 64;
     if(warp == 8 && nT > 0) {
       // ---------------- requests ----------------
@@ -299,7 +333,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
   }
   else {
     // ---------------- softmax: warpgroup t has row tile t, thread i of it row i ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     const int t = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     if(t < nTiles || cut) {
       const int steps = t == 0 ? steps0 : steps1;
@@ -307,6 +341,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
       const uint32_t tS = tmem + t * 128u + lanes, tO = tmem + Sh::O_AT + t * D + lanes, tP = tmem + Sh::P_AT + t * Sh::P_STEP + lanes;
       const float c = x.scale * 1.4426950408889634f;
       const float2 c2 = make_float2(c, c);
+      const float cu = c * (1.0f / 142.0f);
       float ref = -INFINITY, sum = 0.0f;
       bool ok = true;
       for(int i = 0; i < steps; i++) {
@@ -315,11 +350,9 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
         tcFenceAfter();
         const int kind = sKind[j % ST];
-        uint32_t s[4][32];
-#pragma unroll
-        for(int k = 0; k < 4; k++) tmemLd32(tS + 32u * k, s[k]);
-#pragma unroll
-        for(int k = 0; k < 4; k++) tmemLdWaitFor(s[k]);
+        uint32_t s[2][64];
+        tmemLd64Now(tS, s[0]);
+        tmemLd64Now(tS + 64u, s[1]);
         if(Sh::APART) {  // the next scores may come
           tcFenceBefore();
           __syncwarp();
@@ -327,9 +360,9 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         }
         float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for(int k = 0; k < 4; k++)
+        for(int k = 0; k < 2; k++)
 #pragma unroll
-          for(int e = 0; e < 32; e += 2) top[(e / 2) & 3] = max3Nan(top[(e / 2) & 3], __uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1]));
+          for(int e = 0; e < 64; e += 2) top[(e / 2) & 3] = max3Nan(top[(e / 2) & 3], __uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1]));
         const float now = kind == XT_NONE ? -INFINITY : max3Nan(max3Nan(top[0], top[1], top[2]), top[3], top[3]) * c;
         const bool grow = row < a.tileRows && (now > ref + XT_GROW || now != now);
         if(__any_sync(0xffffffffu, grow)) {
@@ -356,14 +389,13 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         }
         const float base = ref == -INFINITY ? 0.0f : -ref;
         const float2 base2 = make_float2(base, base);
+        const float baseU = fmaf(base, 1.0f / 142.0f, 126.0f / 142.0f);  // (t + 126) / 142 lies in [0, 1] as far as t <= 16
         float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         if(Sh::APART && i > 0) {  // the product before has read the probabilities that these replace
           ok = wait(&bO[t], (uint32_t)(i - 1) & 1u);
           if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
           tcFenceAfter();
         }
-        // which pairs of eight take the polynomial
-        constexpr uint32_t poly = Sh::POLY == 3 ? 0x4Au : (Sh::POLY == 2 ? 0x44u : 0u);
         auto exponentials = [&](auto some) {  // some: not every key counts
           const float2* count = reinterpret_cast<const float2*>(sCount + (j % ST) * XT_KEYS);
 #pragma unroll
@@ -371,8 +403,13 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
             uint32_t p[16];
 #pragma unroll
             for(int e = 0; e < 16; e++) {
-              const float2 v = __ffma2_rn(make_float2(__uint_as_float(s[k][2 * e]), __uint_as_float(s[k][2 * e + 1])), c2, base2);
-              const float2 w = ((poly >> (e & 7)) & 1u) ? ex2Poly<T>(v) : make_float2(ex2Approx(v.x), ex2Approx(v.y));
+              const float s0 = __uint_as_float(s[k >> 1][(k & 1) * 32 + 2 * e]), s1 = __uint_as_float(s[k >> 1][(k & 1) * 32 + 2 * e + 1]);
+              float2 w;
+              if((e & 7) == 3) w = ex2Poly<T>(make_float2(fmaSat(s0, cu, baseU), fmaSat(s1, cu, baseU)));
+              else {
+                const float2 v = __ffma2_rn(make_float2(s0, s1), c2, base2);
+                w = make_float2(ex2Approx(v.x), ex2Approx(v.y));
+              }
               part[e & 1] = decltype(some)::value ? __ffma2_rn(w, count[k * 16 + e], part[e & 1]) : __fadd2_rn(part[e & 1], w);
               p[e] = opPack<T>(w.x, w.y);
             }
@@ -417,6 +454,10 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
       else if(nT > 0) ok = ok && wait(&bO[t], (uint32_t)(nT - 1) & 1u);
       if(__any_sync(0xffffffffu, !ok)) ok = false;
       tcFenceAfter();
+      // what the loop does not need is found again instead of kept
+      XaBlock blk = xaBlock(x, a.sp, a.tileRows * a.tilesPerBlock);
+      if(a.longestFirst) blk.b = *sSeq;
+      const int rows = xaRows(x, blk.b, a.G);
       const int r = blk.row0 + (cut ? 0 : t) * a.tileRows + row;
       const bool mine = ok && row < a.tileRows && r < rows;
       const int token = r / a.G, head = blk.kvh * a.G + r - token * a.G;
@@ -514,7 +555,7 @@ XaSplit crossAttnTcSplit(int batch, int qLen, int kLen, int heads, int kvHeads, 
   const int G = heads / kvHeads, tileRows = 128 / G * G;
   const long long rows = (long long)qLen * G, pairs = (rows + 2 * tileRows - 1) / (2 * tileRows) * batch * kvHeads;
   *tilesPerBlock = rows > tileRows && pairs >= smCount() ? 2 : 1;
-  return xaPlanSplit(tileRows * *tilesPerBlock, XT_KEYS, 1024, 1, batch, qLen, kLen, heads, kvHeads, dv);
+  return xaPlanSplit(tileRows * *tilesPerBlock, XT_KEYS, pairs >= smCount() ? INT32_MAX : 1024, 1, batch, qLen, kLen, heads, kvHeads, dv);
 }
 
 cudaError_t launchCrossAttnTc(cudaStream_t st, const CrossAttnArgs& x, const XaSplit& sp, int tilesPerBlock) {
@@ -525,6 +566,7 @@ cudaError_t launchCrossAttnTc(cudaStream_t st, const CrossAttnArgs& x, const XaS
   a.tileTokens = 128 / a.G;
   a.tileRows = a.tileTokens * a.G;
   a.tilesPerBlock = tilesPerBlock;
+  a.longestFirst = x.kLengths && x.batch > 1 && x.batch <= XT_SORT && sp.blocks > (unsigned)smCount();
   const bool wide = x.dq > 64 || x.dv > 64;
   if(x.dt == DT_F16) return wide ? launchTc<__half, 128>(st, a) : launchTc<__half, 64>(st, a);
   return wide ? launchTc<__nv_bfloat16, 128>(st, a) : launchTc<__nv_bfloat16, 64>(st, a);
