@@ -293,7 +293,7 @@ def conv_noalloc(d_in: int, d_weights: int, d_out: int, n: int, nn_x: int, nn_y:
 def matmul(precision: int, m: int, n: int, k: int, x: int, ldx: int, w: int, ldw: int, y: int, ldy: int, bias: int = 0, act: int = 0,
            residual: int = 0, ldr: int = 0, stream: int = 0) -> None:
     """kb_matmul with raw device addresses (ints): y = act(x w^T + bias) + residual.  Enqueues on `stream`."""
-    if lib().kb_matmul(precision, m, n, k, x, ldx, w, ldw, bias, act, residual, ldr, y, ldy, stream):
+    if (_lib or lib()).kb_matmul(precision, m, n, k, x, ldx, w, ldw, bias, act, residual, ldr, y, ldy, stream):
         _check(1, "kb_matmul")
 
 
@@ -301,16 +301,16 @@ def rope(precision: int, batch: int, tokens: int, head_dim: int, rot_dim: int, p
          freq_heads: int, pairs_in_halves: int, q_in: View, q_out: View, q_heads: int, k_in: View = None, k_out: View = None, k_heads: int = 0,
          stream: int = 0) -> None:
     """kb_rope: turns the pairs of q's and k's heads by positions with several axes.  Enqueues on `stream`."""
-    if lib().kb_rope(precision, batch, tokens, head_dim, rot_dim, positions, pos_batch_stride, axes, freqs, freq_heads, pairs_in_halves,
-                     q_in, q_out, q_heads, k_in, k_out, k_heads, stream):
+    if (_lib or lib()).kb_rope(precision, batch, tokens, head_dim, rot_dim, positions, pos_batch_stride, axes, freqs, freq_heads, pairs_in_halves,
+                             q_in, q_out, q_heads, k_in, k_out, k_heads, stream):
         _check(1, "kb_rope")
 
 
 def cross_attention_workspace(precision: int, batch: int, q_len: int, k_len: int, heads: int, kv_heads: int, qk_dim: int, v_dim: int) -> int:
     """Bytes of device memory that kb_cross_attention needs for these sizes."""
     n = ctypes.c_size_t()
-    _check(lib().kb_cross_attention_workspace(precision, batch, q_len, k_len, heads, kv_heads, qk_dim, v_dim, ctypes.byref(n)),
-           "kb_cross_attention_workspace")
+    if (_lib or lib()).kb_cross_attention_workspace(precision, batch, q_len, k_len, heads, kv_heads, qk_dim, v_dim, ctypes.byref(n)):
+        _check(1, "kb_cross_attention_workspace")
     return n.value
 
 
@@ -318,7 +318,7 @@ def cross_attention(precision: int, batch: int, q_len: int, k_len: int, heads: i
                     q: View, k: View, v: View, out: View, q_lengths: int = 0, k_lengths: int = 0, key_mask: int = 0, query_mask: int = 0,
                     workspace: int = 0, workspace_bytes: int = 0, stream: int = 0) -> None:
     """kb_cross_attention: attention of q_len tokens to k_len states.  Enqueues on `stream`."""
-    if lib().kb_cross_attention(precision, batch, q_len, k_len, heads, kv_heads, qk_dim, v_dim, scale, q, k, v, out, q_lengths, k_lengths,
+    if (_lib or lib()).kb_cross_attention(precision, batch, q_len, k_len, heads, kv_heads, qk_dim, v_dim, scale, q, k, v, out, q_lengths, k_lengths,
                                 key_mask, query_mask, workspace, workspace_bytes, stream):
         _check(1, "kb_cross_attention")
 

@@ -7,6 +7,7 @@
 // disappear into the conv kernels; what remains besides convolutions is the gpool reduction, a few
 // per-board matmuls and one elementwise pass per gpool block.
 #include "kb_engine.h"
+#include "kb_ops.h"
 
 #include <cuda.h>
 
@@ -623,12 +624,37 @@ void Engine::emitBlock(const BlockW& b, int C, void* raw, void* act, const BNW* 
       });
     }
     else {
-      if(!attentionFits(X_, Y_, dq, dv))
-        throw std::runtime_error("attention block: a board of " + std::to_string(X_) + "x" + std::to_string(Y_) + " with head sizes " +
-                                 std::to_string(dq) + "/" + std::to_string(dv) + " does not fit the attention kernel's shared memory");
-      addOp("attention simt", 2.0 * S * S * (dq + dv) * H, S * (qkvC + oC) * es, [=](cudaStream_t st, const Geom& g) {
-        return launchAttention(st, dt, qkv, qkvC, 0, qC, qC + kC, H, Hkv, dq, dv, mask, attn, oC, g, relBiasDev, relY, relX);
-      });
+      if(!attentionFits(X_, Y_, dq, dv)) {
+        // boards whose keys and values do not fit a block's shared memory: the attention of kb_cross_attention over the rows of the
+        // padded boards, whose padding the mask leaves out
+        if(relBiasDev || dq > 256 || dv > 256)
+          throw std::runtime_error("attention block: a board of " + std::to_string(X_) + "x" + std::to_string(Y_) + " with head sizes " +
+                                   std::to_string(dq) + "/" + std::to_string(dv) + (relBiasDev ? " and a relative-position bias" : "") +
+                                   " does not fit the attention kernel's shared memory");
+        // planned for the handle's largest batch whatever the batch, so that a position's result does not depend on those beside it
+        const int planBatch = maxBatch_, boardRows = makeGeom(X_, Y_, 1).PB;
+        const size_t room = crossAttnWorkspace(dt, planBatch, boardRows, boardRows, H, Hkv, dq, dv);
+        void* workspace = room > 0 ? scratch("tfAttnParts" + d, room) : nullptr;
+        int* status = statusWord_;
+        addOp("attention any board", 2.0 * S * S * (dq + dv) * H, S * (qkvC + oC) * es, [=](cudaStream_t st, const Geom& g) {
+          CrossAttnArgs a = {};
+          a.dt = dt; a.batch = g.n; a.planBatch = planBatch; a.qLen = g.PB; a.kLen = g.PB; a.heads = H; a.kvHeads = Hkv; a.dq = dq; a.dv = dv;
+          a.scale = 1.0f / sqrtf((float)dq);
+          auto at = [&](int c) { return static_cast<const char*>(qkv) + (size_t)c * (dt == DT_F32 ? 4 : 2); };
+          const int64_t boards = (int64_t)g.PB * qkvC;
+          a.q = at(0); a.qB = boards; a.qT = qkvC; a.qH = dq;
+          a.k = at(qC); a.kB = boards; a.kT = qkvC; a.kH = dq;
+          a.v = at(qC + kC); a.vB = boards; a.vT = qkvC; a.vH = dv;
+          a.out = attn; a.oB = (int64_t)g.PB * oC; a.oT = oC; a.oH = dv;
+          a.keyMask = mask; a.queryMask = mask; a.workspace = workspace; a.status = status;
+          return launchCrossAttn(st, a);
+        });
+      }
+      else {
+        addOp("attention simt", 2.0 * S * S * (dq + dv) * H, S * (qkvC + oC) * es, [=](cudaStream_t st, const Geom& g) {
+          return launchAttention(st, dt, qkv, qkvC, 0, qC, qC + kC, H, Hkv, dq, dv, mask, attn, oC, g, relBiasDev, relY, relX);
+        });
+      }
     }
     ConvW outW = matmulsAsConv({&b.out});
     ConvDev co = makeConv({&outW}, attn, oC, oC, nextC);

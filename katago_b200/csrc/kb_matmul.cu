@@ -33,16 +33,20 @@ __device__ __forceinline__ void matmulStore(const MatmulArgs& a, int m, int n, f
   ((T*)a.y)[(int64_t)m * a.ldy + n] = OpType<T>::from(v);
 }
 
-// VEC: rows on 16-byte boundaries and K in whole vectors.  KG: groups of 256 threads that share a slice's channels, their sums added
-// in order at the end: a tile alone on its SM needs more than eight warps to cover the latency of its shared-memory loads
-// (1083 x 362 x 361: 26 us with one group).
-template <int BM, int BN, bool VEC, int KG>
-__global__ void __launch_bounds__(256 * KG) matmulF32Kernel(const MatmulArgs a) {
-  constexpr int BK = 32, PITCH = BK + 4, STAGES = 3, TM = BM / 16, TN = BN / 16;  // 8 rows of 144 bytes start in 8 different bank groups
+// TM x TN outputs per thread: a shared-memory load of 16 bytes per lane is three passes of the shared memory whatever lanes it
+// repeats for, so eight by eight outputs (16 loads for 128 packed FMAs) are needed for the FMA units to be what bounds it.  KG: groups
+// of threads that share a slice's channels and add their sums in order at the end, so that a small tile has threads of that kind
+// enough (1083 x 362 x 361, 64 x 48 tiles, one to an SM: 26 us with 4 x 3 outputs from 256 threads, 19 us from 1024).
+// VEC: rows on 16-byte boundaries and K in whole vectors.
+template <int BM, int BN, int TM, int TN, int KG, bool VEC>
+__global__ void __launch_bounds__(BM / TM * (BN / TN) * KG) matmulF32Kernel(const MatmulArgs a) {
+  constexpr int BK = 32, PITCH = BK + 4, STAGES = 3;  // 8 rows of 144 bytes start in 8 different bank groups
+  constexpr int TX = BN / TN, TY = BM / TM, GROUP = TX * TY, THREADS = GROUP * KG;
+  static_assert(GROUP % 32 == 0 && TX % 8 == 0 && TY % 4 == 0 && BK % (4 * KG) == 0, "a warp is four rows by eight columns of one group");
   extern __shared__ float4 smem4[];
   float* sm = reinterpret_cast<float*>(smem4);
-  const int tid = threadIdx.x, kg = tid >> 8;
-  const int tx = ((tid >> 5) & 1) * 8 + (tid & 7), ty = ((tid & 255) >> 6) * 4 + ((tid >> 3) & 3);  // a warp: four rows by eight columns
+  const int tid = threadIdx.x, kg = tid / GROUP, warp = (tid % GROUP) >> 5, lane = tid & 31;
+  const int tx = warp % (TX / 8) * 8 + (lane & 7), ty = warp / (TX / 8) * 4 + (lane >> 3);
   const int tilesN = (a.N + BN - 1) / BN;
   const int m0 = (int)(blockIdx.x / tilesN) * BM, n0 = (int)(blockIdx.x % tilesN) * BN;
   const float* x = (const float*)a.x;
@@ -54,7 +58,7 @@ __global__ void __launch_bounds__(256 * KG) matmulF32Kernel(const MatmulArgs a) 
     float* dst = sm + (s % STAGES) * (BM + BN) * PITCH;
     constexpr int E = VEC ? 4 : 1, PER = BK / E;
 #pragma unroll
-    for(int i = tid; i < (BM + BN) * PER; i += 256 * KG) {
+    for(int i = tid; i < (BM + BN) * PER; i += THREADS) {
       const int r = i / PER, k = s * BK + (i % PER) * E;
       const bool isX = r < BM;
       const int row = isX ? m0 + r : n0 + r - BM;
@@ -80,58 +84,56 @@ __global__ void __launch_bounds__(256 * KG) matmulF32Kernel(const MatmulArgs a) 
     __syncthreads();  // slice s is there, and everyone is done with the slot of slice s - 1
     if(s + STAGES - 1 < steps) load(s + STAGES - 1);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const float* sA = sm + (s % STAGES) * (BM + BN) * PITCH + ty * PITCH;
-    const float* sB = sm + (s % STAGES) * (BM + BN) * PITCH + (BM + tx) * PITCH;
-    // the operands of four channels are loaded while those before are multiplied, if there are registers for both
-    constexpr int AHEAD = TM * TN <= 32 ? 1 : 0;
-    float4 av[1 + AHEAD][TM], bv[1 + AHEAD][TN];
-    auto operands = [&](int b, int k) {
-#pragma unroll
-      for(int i = 0; i < TM; i++) av[b][i] = *reinterpret_cast<const float4*>(sA + 16 * i * PITCH + k);
-#pragma unroll
-      for(int j = 0; j < TN; j++) bv[b][j] = *reinterpret_cast<const float4*>(sB + 16 * j * PITCH + k);
-    };
-    if(AHEAD) operands(0, kg * (BK / KG));
+    const float* sA = sm + (s % STAGES) * (BM + BN) * PITCH + ty * PITCH + kg * (BK / KG);
+    const float* sB = sm + (s % STAGES) * (BM + BN) * PITCH + (BM + tx) * PITCH + kg * (BK / KG);
 #pragma unroll
     for(int k = 0; k < BK / KG; k += 4) {
-      const int b = AHEAD ? (k / 4) & 1 : 0;
-      if(!AHEAD) operands(0, kg * (BK / KG) + k);
-      else if(k + 4 < BK / KG) operands((b ^ 1) * AHEAD, kg * (BK / KG) + k + 4);
+      float4 av[TM], bv[TN];
+#pragma unroll
+      for(int i = 0; i < TM; i++) av[i] = *reinterpret_cast<const float4*>(sA + TY * i * PITCH + k);
+#pragma unroll
+      for(int j = 0; j < TN; j++) bv[j] = *reinterpret_cast<const float4*>(sB + TX * j * PITCH + k);
 #pragma unroll
       for(int i = 0; i < TM; i++)
 #pragma unroll
-        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(make_float2(av[b][i].x, av[b][i].y), make_float2(bv[b][j].x, bv[b][j].y), acc[i][j]);
+        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(make_float2(av[i].x, av[i].y), make_float2(bv[j].x, bv[j].y), acc[i][j]);
 #pragma unroll
       for(int i = 0; i < TM; i++)
 #pragma unroll
-        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(make_float2(av[b][i].z, av[b][i].w), make_float2(bv[b][j].z, bv[b][j].w), acc[i][j]);
+        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(make_float2(av[i].z, av[i].w), make_float2(bv[j].z, bv[j].w), acc[i][j]);
     }
   }
   if(KG > 1) {
-    static_assert((KG - 1) * TM * TN * 256 <= STAGES * (BM + BN) * PITCH, "the groups' sums take the place of the slices");
+    static_assert((KG - 1) * TM * TN * GROUP <= STAGES * (BM + BN) * PITCH, "the groups' sums take the place of the slices");
     __syncthreads();
     if(kg > 0)
 #pragma unroll
       for(int i = 0; i < TM; i++)
 #pragma unroll
-        for(int j = 0; j < TN; j++) sm[(((kg - 1) * TM + i) * TN + j) * 256 + (tid & 255)] = acc[i][j].x + acc[i][j].y;
+        for(int j = 0; j < TN; j++) sm[(((kg - 1) * TM + i) * TN + j) * GROUP + tid % GROUP] = acc[i][j].x + acc[i][j].y;
     __syncthreads();
-    if(kg > 0) return;
 #pragma unroll
-    for(int g = 0; g < KG - 1; g++)
+    for(int i = 0; i < TM; i++) {
+      const int m = m0 + ty + TY * i;
 #pragma unroll
-      for(int i = 0; i < TM; i++)
+      for(int j = 0; j < TN; j++) {
+        const int n = n0 + tx + TX * j;
+        if(kg > 0) continue;
+        float v = acc[i][j].x + acc[i][j].y;
 #pragma unroll
-        for(int j = 0; j < TN; j++) acc[i][j].x += sm[((g * TM + i) * TN + j) * 256 + tid];
+        for(int g = 0; g < KG - 1; g++) v += sm[((g * TM + i) * TN + j) * GROUP + tid];
+        if(m < a.M && n < a.N) matmulStore<float>(a, m, n, v);
+      }
+    }
+    return;
   }
 #pragma unroll
   for(int i = 0; i < TM; i++) {
-    const int m = m0 + ty + 16 * i;
-    if(m >= a.M) continue;
+    const int m = m0 + ty + TY * i;
 #pragma unroll
     for(int j = 0; j < TN; j++) {
-      const int n = n0 + tx + 16 * j;
-      if(n < a.N) matmulStore<float>(a, m, n, acc[i][j].x + acc[i][j].y);
+      const int n = n0 + tx + TX * j;
+      if(m < a.M && n < a.N) matmulStore<float>(a, m, n, acc[i][j].x + acc[i][j].y);
     }
   }
 }
@@ -394,8 +396,10 @@ template <typename T, int V> struct TileForms {
 };
 template <int V> struct TileForms<float, V> {
   static cudaError_t launch(cudaStream_t st, const MatmulArgs& a) {
-    static const TileForm forms[] = {{128, 128, 1.0, matmulF32Kernel<128, 128, V == 4, 1>, 256}, {128, 64, 1.15, matmulF32Kernel<128, 64, V == 4, 1>, 256}, 
-                                     {64, 64, 1.3, matmulF32Kernel<64, 64, V == 4, 2>, 512},                                     {64, 48, 1.35, matmulF32Kernel<64, 48, V == 4, 4>, 1024}, {32, 32, 1.9, matmulF32Kernel<32, 32, V == 4, 4>, 1024}};
+    constexpr bool VEC = V == 4;
+    static const TileForm forms[] = {{128, 128, 1.0, matmulF32Kernel<128, 128, 8, 8, 1, VEC>, 256}, {128, 64, 1.1, matmulF32Kernel<128, 64, 8, 8, 2, VEC>, 256},
+                                     {64, 64, 1.35, matmulF32Kernel<64, 64, 8, 8, 4, VEC>, 256},    {64, 48, 1.4, matmulF32Kernel<64, 48, 8, 6, 4, VEC>, 256},
+                                     {32, 32, 2.0, matmulF32Kernel<32, 32, 4, 4, 4, VEC>, 256}};
     static SharedMemoryOptIn optIn[5];
     return launchTiles(st, a, forms, optIn, [](int bm, int bn) -> size_t { return (size_t)3 * (bm + bn) * 36 * 4; });
   }

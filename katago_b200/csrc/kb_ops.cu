@@ -24,9 +24,9 @@ size_t elementSize(int precision, const char* op) {
 
 // Where the current device's kernels find it: device memory of this device (or managed memory).
 void checkPointer(const char* op, const char* name, const void* p, size_t align) {
-  const std::string who = std::string(op) + ": " + name;
-  if(p == nullptr) refuse(who + " is NULL");
-  if((uintptr_t)p % align != 0) refuse(who + " is not aligned to its elements of " + std::to_string(align) + " bytes");
+  auto who = [&]() { return std::string(op) + ": " + name; };
+  if(p == nullptr) refuse(who() + " is NULL");
+  if((uintptr_t)p % align != 0) refuse(who() + " is not aligned to its elements of " + std::to_string(align) + " bytes");
   typedef CUresult (*GetAttributesFn)(unsigned int, CUpointer_attribute*, void**, CUdeviceptr);
   static const GetAttributesFn get = []() -> GetAttributesFn {
     void* f = nullptr;
@@ -34,16 +34,16 @@ void checkPointer(const char* op, const char* name, const void* p, size_t align)
     if(cudaGetDriverEntryPoint("cuPointerGetAttributes", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
     return reinterpret_cast<GetAttributesFn>(f);
   }();
-  if(!get) refuse(who + ": no CUDA device");
+  if(!get) refuse(who() + ": no CUDA device");
   unsigned int type = 0, managed = 0;
   int dev = -1, cur = -1;
   CUpointer_attribute ask[3] = {CU_POINTER_ATTRIBUTE_MEMORY_TYPE, CU_POINTER_ATTRIBUTE_IS_MANAGED, CU_POINTER_ATTRIBUTE_DEVICE_ORDINAL};
   void* into[3] = {&type, &managed, &dev};
-  if(get(3, ask, into, (CUdeviceptr)(uintptr_t)p) != CUDA_SUCCESS) refuse(who + " could not be looked up");
+  if(get(3, ask, into, (CUdeviceptr)(uintptr_t)p) != CUDA_SUCCESS) refuse(who() + " could not be looked up");
   if(managed) return;
-  if(type != CU_MEMORYTYPE_DEVICE) refuse(who + " is not device memory");
+  if(type != CU_MEMORYTYPE_DEVICE) refuse(who() + " is not device memory");
   cudaCheck(cudaGetDevice(&cur), "cudaGetDevice");
-  if(dev != cur) refuse(who + " lies on device " + std::to_string(dev) + ", the current device is " + std::to_string(cur));
+  if(dev != cur) refuse(who() + " lies on device " + std::to_string(dev) + ", the current device is " + std::to_string(cur));
 }
 
 // A tensor [n[0]][n[1]][n[2]][width] with strides in elements; the last dimension is contiguous.

@@ -55,6 +55,7 @@ cudaError_t launchRopeAxes(cudaStream_t st, const RopeArgs& a);
 // ---- attention to states of another length ----
 struct CrossAttnArgs {
   int dt, batch, qLen, kLen, heads, kvHeads, dq, dv;
+  int planBatch;  // the batch that the cutting of rows and keys is planned for; 0: this one (the workspace is planBatch's)
   float scale;
   const void* q; int64_t qB, qT, qH;
   const void* k; int64_t kB, kT, kH;

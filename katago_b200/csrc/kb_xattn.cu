@@ -420,8 +420,9 @@ size_t crossAttnWorkspace(int dt, int batch, int qLen, int kLen, int heads, int 
 
 cudaError_t launchCrossAttn(cudaStream_t st, const CrossAttnArgs& a) {
   if(a.batch == 0 || a.qLen == 0) return cudaSuccess;
-  Plan p = planFor(a.dt, a.batch, a.qLen, a.kLen, a.heads, a.kvHeads, a.dq, a.dv);
+  Plan p = planFor(a.dt, a.planBatch > 0 ? a.planBatch : a.batch, a.qLen, a.kLen, a.heads, a.kvHeads, a.dq, a.dv);
   XaSplit& sp = p.sp;
+  sp.blocks = (unsigned)((long long)a.batch * a.kvHeads * sp.rowTiles * sp.parts);
   if(p.kind != Plan::SIMT && !crossAttnAligned(a)) {
     p.kind = Plan::SIMT;
     const int rows = simtRows(a.qLen, a.heads, a.kvHeads);

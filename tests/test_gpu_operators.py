@@ -484,6 +484,40 @@ def test_blocks_from_several_threads_at_once():
         assert torch.equal(a, b)
 
 
+# ---- nets on boards that only this attention takes ----
+
+@pytest.mark.parametrize("ylen,xlen", [(22, 22), (19, 25), (37, 20)])
+def test_transformer_nets_on_large_boards(ylen, xlen, oracle):
+    """Boards whose keys and values do not fit a block's shared memory (above about 19x19), against the oracle; a position's result does
+    not depend on the batch that it is evaluated in."""
+    import numpy as np
+
+    from katago_b200 import modelfile as mf
+    from tests.test_gpu_parity import _assert_fp32_close, _assert_reduced_close, _rect_positions
+    sp, gl = _rect_positions(3, ylen, xlen, seed=ylen * 100 + xlen)
+    mask = sp[..., 0].reshape(3, -1)
+    for tree in (mf.make_transformer(seed=61, layers=2), mf.make_transformer(seed=9, layers=2, d=64, heads=2, head_dim=32, ffn=96, rope="fixed")):
+        blob = mf.to_blob(tree)
+        ref = oracle.OracleModel(blob, nn_x=xlen, nn_y=ylen).forward(sp, gl)
+        for prec in (capi.PRECISION_FP32, capi.PRECISION_FP16, capi.PRECISION_BF16):
+            h = capi.Handle(capi.Model(blob), 3, nn_x=xlen, nn_y=ylen, precision=prec)
+            got = h.forward(sp, gl)
+            one = h.forward(sp[1:2], gl[1:2])
+            h.close()
+            if prec == capi.PRECISION_FP32:
+                _assert_fp32_close(got, ref, mask)
+            elif prec == capi.PRECISION_FP16:
+                _assert_reduced_close(got, ref, mask)
+            for key in one:
+                assert np.array_equal(one[key][0], got[key][1]), key
+
+
+def test_a_large_board_with_a_relative_position_bias_is_refused():
+    from katago_b200 import modelfile as mf
+    with pytest.raises(capi.KBError, match="larger than the relative-position bias table|relative-position bias"):
+        capi.Handle(capi.Model(mf.to_blob(mf.make_transformer_relbias(seed=62, layers=1))), 1, nn_x=22, nn_y=22, precision=capi.PRECISION_FP16)
+
+
 # ---- refusals that need a device ----
 
 def test_refusals_of_pointers_and_overlaps():
