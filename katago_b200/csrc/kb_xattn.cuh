@@ -44,9 +44,8 @@ __device__ __forceinline__ int xaKeys(const CrossAttnArgs& a, int b) {
   return a.kLengths ? max(0, min(a.kLengths[b], a.kLen)) : a.kLen;
 }
 // Parts of one row tile are neighbours in the grid, then the row tiles of a key head (they share its K and V in L2).
-__device__ __forceinline__ XaBlock xaBlock(const CrossAttnArgs& a, const XaSplit& sp, int rowsPerBlock) {
+__device__ __forceinline__ XaBlock xaBlock(const CrossAttnArgs& a, const XaSplit& sp, int rowsPerBlock, unsigned i = blockIdx.x) {
   XaBlock k;
-  unsigned i = blockIdx.x;
   k.part = i % sp.parts; i /= sp.parts;
   k.row0 = (int)(i % sp.rowTiles) * rowsPerBlock; i /= sp.rowTiles;
   k.kvh = i % a.kvHeads;

@@ -43,6 +43,8 @@ MATMULS = [
     (1, 1, 1), (1, 64, 64), (1, 4096, 384), (2, 7, 1000), (3, 129, 72), (4, 512, 4096), (5, 50, 33), (8, 257, 136), (9, 64, 64), (16, 256, 128),
     (17, 40, 24), (31, 1000, 520), (64, 384, 384), (65, 96, 200), (127, 128, 64), (128, 256, 512), (129, 130, 131), (300, 8, 1536), (361, 384, 1024),
     (700, 1152, 384), (1083, 362, 361), (1500, 512, 65), (40, 2048, 2048), (2048, 264, 264),
+    # several tiles per SM, the last ones partial in both directions; K cut over a cluster with rows of x in two tiles
+    (5000, 1000, 200), (20000, 136, 72), (2100, 2000, 40), (2100, 2001, 33), (200, 300, 2600),
 ]
 
 
@@ -277,6 +279,34 @@ def test_attention_left_out_keys_may_hold_anything(dtype, b, n, m, h, hk, dq, dv
     for i in range(b):
         if dead[i]:
             assert (out[i, : int(tokens[i])] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("b,n,m,h,hk,dq,dv", [(40, 300, 130, 4, 4, 64, 64), (40, 300, 200, 12, 4, 128, 128), (75, 257, 129, 2, 2, 64, 40), (30, 260, 300, 10, 5, 96, 128),
+                                              (150, 1, 900, 4, 2, 64, 64), (150, 20, 300, 2, 2, 64, 64)])
+@pytest.mark.parametrize("ragged", (False, True))
+def test_attention_with_more_blocks_than_sms(dtype, ragged, b, n, m, h, hk, dq, dv):
+    """Blocks of two row tiles, the last round's apart, sequences in the order of their lengths."""
+    g, q, k, v = attention_inputs(dtype, b, n, m, h, hk, dq, dv, ragged)
+    lengths = mask = tokens = None
+    if ragged:
+        lengths = torch.randint(0, m + 1, (b,), generator=g, device="cuda").to(torch.int32)
+        lengths[:3] = torch.tensor([0, m, 1])
+        mask = (torch.rand(b, m, generator=g, device="cuda") < 0.7).float()
+        mask[5, :] = 0
+        mask[6, :128] = 0
+        tokens = torch.randint(0, n + 1, (b,), generator=g, device="cuda").to(torch.int32)
+        tokens[0] = n
+        left_out = (torch.arange(m, device="cuda") >= lengths[:, None]) | (mask == 0)
+        k[left_out], v[left_out] = NAN, float("inf")
+    want, bound = attention_reference(dtype, q, k, v, dq ** -0.5, k_lengths=lengths, key_mask=mask)
+    out = torch.full_like(empty_out(q, v), 7.0)
+    attend(dtype, q, k, v, out, dq ** -0.5, tokens, lengths, mask)
+    if tokens is not None:
+        behind = torch.arange(n, device="cuda") >= tokens[:, None]
+        assert (out[behind] == 7.0).all()
+        out[behind], want[behind], bound[behind] = 0, 0, 0
+    assert_within(out.flatten(0, 1), want.flatten(0, 1), bound.flatten(0, 1))
 
 
 @pytest.mark.parametrize("dtype", ALL)
