@@ -104,26 +104,20 @@ __global__ void __launch_bounds__(BM / TM * (BN / TN) * KG) matmulF32Kernel(cons
     }
   }
   if(KG > 1) {
-    static_assert((KG - 1) * TM * TN * GROUP <= STAGES * (BM + BN) * PITCH, "the groups' sums take the place of the slices");
-    __syncthreads();
-    if(kg > 0)
-#pragma unroll
-      for(int i = 0; i < TM; i++)
-#pragma unroll
-        for(int j = 0; j < TN; j++) sm[(((kg - 1) * TM + i) * TN + j) * GROUP + tid % GROUP] = acc[i][j].x + acc[i][j].y;
+    // the groups' sums [group][BM][BN] take the place of the slices; all threads add up and finish a share of the outputs
     __syncthreads();
 #pragma unroll
-    for(int i = 0; i < TM; i++) {
-      const int m = m0 + ty + TY * i;
+    for(int i = 0; i < TM; i++)
 #pragma unroll
-      for(int j = 0; j < TN; j++) {
-        const int n = n0 + tx + TX * j;
-        if(kg > 0) continue;
-        float v = acc[i][j].x + acc[i][j].y;
+      for(int j = 0; j < TN; j++) sm[(kg * BM + ty + TY * i) * BN + tx + TX * j] = acc[i][j].x + acc[i][j].y;
+    __syncthreads();
+    for(int i = tid; i < BM * BN; i += THREADS) {
+      const int m = m0 + i / BN, n = n0 + i % BN;
+      if(m >= a.M || n >= a.N) continue;
+      float v = sm[i];
 #pragma unroll
-        for(int g = 0; g < KG - 1; g++) v += sm[((g * TM + i) * TN + j) * GROUP + tid];
-        if(m < a.M && n < a.N) matmulStore<float>(a, m, n, v);
-      }
+      for(int g = 1; g < KG; g++) v += sm[g * BM * BN + i];
+      matmulStore<float>(a, m, n, v);
     }
     return;
   }
@@ -367,8 +361,9 @@ struct TileForm {
   double per;  // cost of an output, relative
   void (*run)(const MatmulArgs);
   int threads;
+  size_t smem;
 };
-template <int N> cudaError_t launchTiles(cudaStream_t st, const MatmulArgs& a, const TileForm (&forms)[N], SharedMemoryOptIn (&optIn)[N], size_t (*smem)(int, int)) {
+template <int N> cudaError_t launchTiles(cudaStream_t st, const MatmulArgs& a, const TileForm (&forms)[N], SharedMemoryOptIn (&optIn)[N]) {
   int pick = 0;
   double best = 0;
   long long count = 0;
@@ -378,7 +373,7 @@ template <int N> cudaError_t launchTiles(cudaStream_t st, const MatmulArgs& a, c
     if(i == 0 || cost < best) { best = cost; pick = i; count = tiles; }
   }
   if(count >= 1LL << 31) return cudaErrorInvalidValue;
-  const size_t bytes = smem(forms[pick].bm, forms[pick].bn);
+  const size_t bytes = forms[pick].smem;
   if(bytes > 48 * 1024) {
     const cudaError_t e = optIn[pick]((const void*)forms[pick].run, (int)bytes);
     if(e != cudaSuccess) return e;
@@ -388,20 +383,21 @@ template <int N> cudaError_t launchTiles(cudaStream_t st, const MatmulArgs& a, c
 template <typename T, int V> struct TileForms {
   static cudaError_t launch(cudaStream_t st, const MatmulArgs& a) {
     constexpr int VT = V > 4 ? 4 : V;  // elements of an access: four threads per staged row
-    static const TileForm forms[] = {{128, 128, 1.0, matmulTileKernel<T, 128, 128, VT>, 256}, {64, 64, 1.25, matmulTileKernel<T, 64, 64, VT>, 256},
-                                     {64, 48, 1.3, matmulTileKernel<T, 64, 48, VT>, 256}, {32, 32, 2.0, matmulTileKernel<T, 32, 32, VT>, 256}};
+    static const TileForm forms[] = {{128, 128, 1.0, matmulTileKernel<T, 128, 128, VT>, 256, 0}, {64, 64, 1.25, matmulTileKernel<T, 64, 64, VT>, 256, 0},
+                                     {64, 48, 1.3, matmulTileKernel<T, 64, 48, VT>, 256, 0}, {32, 32, 2.0, matmulTileKernel<T, 32, 32, VT>, 256, 0}};
     static SharedMemoryOptIn optIn[4];
-    return launchTiles(st, a, forms, optIn, [](int, int) -> size_t { return 0; });
+    return launchTiles(st, a, forms, optIn);
   }
 };
 template <int V> struct TileForms<float, V> {
   static cudaError_t launch(cudaStream_t st, const MatmulArgs& a) {
-    constexpr bool VEC = V == 4;
-    static const TileForm forms[] = {{128, 128, 1.0, matmulF32Kernel<128, 128, 8, 8, 1, VEC>, 256}, {128, 64, 1.1, matmulF32Kernel<128, 64, 8, 8, 2, VEC>, 256},
-                                     {64, 64, 1.35, matmulF32Kernel<64, 64, 8, 8, 4, VEC>, 256},    {64, 48, 1.4, matmulF32Kernel<64, 48, 8, 6, 4, VEC>, 256},
-                                     {32, 32, 2.0, matmulF32Kernel<32, 32, 4, 4, 4, VEC>, 256}};
+    static const TileForm forms[] = {form<128, 128, 8, 8, 1>(1.0), form<128, 64, 8, 8, 2>(1.1), form<64, 64, 8, 8, 4>(1.35), form<64, 48, 8, 6, 4>(1.4), form<32, 32, 4, 4, 4>(2.0)};
     static SharedMemoryOptIn optIn[5];
-    return launchTiles(st, a, forms, optIn, [](int bm, int bn) -> size_t { return (size_t)3 * (bm + bn) * 36 * 4; });
+    return launchTiles(st, a, forms, optIn);
+  }
+  template <int BM, int BN, int TM, int TN, int KG> static TileForm form(double per) {
+    const size_t slices = (size_t)3 * (BM + BN) * 36 * 4, sums = KG > 1 ? (size_t)KG * BM * BN * 4 : 0;
+    return {BM, BN, per, matmulF32Kernel<BM, BN, TM, TN, KG, V == 4>, BM / TM * (BN / TN) * KG, std::max(slices, sums)};
   }
 };
 

@@ -40,9 +40,20 @@ template <typename T, int V> struct OpVec {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<word*>(p) = w; }
 };
 
-// Activations: exact functions for fp32 results, the special-function forms of the convolutions' epilogues for 16-bit ones
-// (their error is far below the rounding of the result).
-template <typename T> __device__ __forceinline__ float opAct(float v, int act) { return sizeof(T) == 4 ? applyActF(v, act) : fastAct(v, act); }
+// Activations: library functions for fp32 results, the special-function forms of the convolutions' epilogues for 16-bit ones (their
+// error is far below the rounding of the result).  mish(x) = x tanh(log(1 + e^x)) = x (n^2 + 2n) / (n^2 + 2n + 2) with n = e^x:
+// nothing cancels, and one exponential and a division take the place of exp, log1p and tanh.
+__device__ __forceinline__ float opMish(float x, float arg) {
+  const float n = expf(fminf(arg, 30.0f));  // the quotient is 1 from about 9 on
+  const float m = n * (n + 2.0f);
+  return x * (m / (m + 2.0f));
+}
+template <typename T> __device__ __forceinline__ float opAct(float v, int act) {
+  if(sizeof(T) != 4) return fastAct(v, act);
+  if(act == KB_ACT_MISH) return opMish(v, v);
+  if(act == KB_ACT_MISH_SCALE8) return opMish(v, 8.0f * v);
+  return applyActF(v, act);
+}
 
 // Bounded wait of a role of these kernels (about 2 s).  A wait that runs out raises the abort flag and leaves `code` in the status
 // word, which is page-locked host memory (hence a plain store); it returns false, as does one that finds the flag raised, and

@@ -40,8 +40,8 @@ __device__ __forceinline__ unsigned long long turnFraction(float freq) {
 constexpr int ROPE_TABLE = 4096;
 
 // MODE 0: scalar pairs (any alignment), 1: V elements = V/2 adjacent pairs per access, 2: halves, V pairs per two accesses
-template <typename T, int MODE, int V>
-__global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const RopeArgs a, int chunks, int rotChunks, int headsPerItem, long long items) {
+template <typename T, int MODE, int V, bool COPY>
+__global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const RopeArgs a, int chunks, int copies, int headsPerItem, long long items) {
   extern __shared__ unsigned long long sTurn[];  // [freqHeads][pairs][axes], or nothing
   gridDepLaunch();
   gridDepWait();
@@ -70,16 +70,6 @@ __global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const R
     T* kOut = (T*)a.k.out + b * a.k.outB + t * a.k.outT;
     auto in = [&](int h) { return h < a.q.heads ? qIn + h * a.q.inH : kIn + (h - a.q.heads) * a.k.inH; };
     auto out = [&](int h) { return h < a.q.heads ? qOut + h * a.q.outH : kOut + (h - a.q.heads) * a.k.outH; };
-    if(c >= rotChunks) {  // channels without a position
-      constexpr int W = MODE == 0 ? 1 : V;
-      const int e = a.rot + (c - rotChunks) * W;
-      for(int h = h0; h < h1; h++) {
-        OpVec<T, W> v;
-        v.load(in(h) + e);
-        v.store(out(h) + e);
-      }
-      continue;
-    }
     float cs[P], sn[P];
     int have = -1;  // the table whose angles they are
     const int32_t* pos = a.positions + b * a.posB + (long long)t * a.axes;
@@ -141,6 +131,31 @@ __global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const R
       }
     }
   }
+  if(!COPY) return;
+  // channels without a position: `copies` vectors of every head, in items of their own, so that a warp has either kind (7 x 1083 tokens
+  // of 10 heads, 48 of 80 channels turned, fp32: 15.9 us; 23.7 us with both kinds in a warp)
+  constexpr int W = MODE == 0 ? 1 : V, N = 4;  // items in flight
+  const long long all = (long long)a.batch * a.tokens * totalHeads * copies, step = (long long)gridDim.x * blockDim.x;
+  for(long long item = (long long)blockIdx.x * blockDim.x + threadIdx.x; item < all; item += N * step) {
+    OpVec<T, W> v[N];
+    T* to[N];
+#pragma unroll
+    for(int u = 0; u < N; u++) {
+      const long long i = item + u * step;
+      to[u] = nullptr;
+      if(i >= all) continue;
+      const long long rest = i / copies, bt = rest / totalHeads;
+      const int e = a.rot + (int)(i - rest * copies) * W, h = (int)(rest - bt * totalHeads);
+      const int b = (int)(bt / a.tokens), t = (int)(bt - (long long)b * a.tokens);
+      const RopeHeads& x = h < a.q.heads ? a.q : a.k;
+      const int hh = h < a.q.heads ? h : h - a.q.heads;
+      v[u].load((const T*)x.in + b * x.inB + t * x.inT + hh * x.inH + e);
+      to[u] = (T*)x.out + b * x.outB + t * x.outT + hh * x.outH + e;
+    }
+#pragma unroll
+    for(int u = 0; u < N; u++)
+      if(to[u]) v[u].store(to[u]);
+  }
 }
 
 template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a) {
@@ -155,8 +170,8 @@ template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a)
   const bool vec = aligned(a.q) && aligned(a.k) && a.rot % unit == 0 && a.dim % V == 0;
   // in place the channels behind the rotated ones stay as they are
   const bool copy = (a.q.heads && a.q.in != a.q.out) || (a.k.heads && a.k.in != a.k.out);
-  const int rotChunks = vec ? a.rot / unit : a.rot / 2;
-  const int chunks = rotChunks + (copy ? (vec ? (a.dim - a.rot) / V : a.dim - a.rot) : 0);
+  const int chunks = vec ? a.rot / unit : a.rot / 2;
+  const int copies = copy ? (vec ? (a.dim - a.rot) / V : a.dim - a.rot) : 0;
   const int heads = a.q.heads + a.k.heads;
   const long long perHead = (long long)a.batch * a.tokens * chunks;
   if(perHead == 0 || heads == 0) return cudaSuccess;
@@ -173,9 +188,11 @@ template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a)
   // 664 MB: 124 us, 5.4 TB/s; 303 us with three, spilled).
   const long long blocks = std::min<long long>((items + 255) / 256, 6LL * smCount());
   const dim3 grid((unsigned)blocks), block(256);
-  if(!vec) return launchDependent(ropeAxesKernel<T, 0, 1>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
-  if(a.halves) return launchDependent(ropeAxesKernel<T, 2, V>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
-  return launchDependent(ropeAxesKernel<T, 1, V>, grid, block, smem, st, a, chunks, rotChunks, headsPerItem, items);
+  auto run = [&](auto kernel) { return launchDependent(kernel, grid, block, smem, st, a, chunks, copies, headsPerItem, items); };
+  // (without channels to copy, a kernel without that loop: it costs the other one registers, 128 x 361 tokens 27.7 -> 32 us)
+  if(!vec) return copies ? run(ropeAxesKernel<T, 0, 1, true>) : run(ropeAxesKernel<T, 0, 1, false>);
+  if(a.halves) return copies ? run(ropeAxesKernel<T, 2, V, true>) : run(ropeAxesKernel<T, 2, V, false>);
+  return copies ? run(ropeAxesKernel<T, 1, V, true>) : run(ropeAxesKernel<T, 1, V, false>);
 }
 
 }  // namespace
