@@ -186,7 +186,9 @@ const char* kb_conv_noalloc_last_error(void);
  *     device are refused.  Elements have the type that `precision` (KB_PRECISION_*) names, sums are held in fp32, a result is
  *     rounded once;
  *   - strides count elements and may be anything from 0 up for inputs (0 repeats); the innermost dimension is contiguous;
- *     elements of an output must not coincide, and an output must not overlap an input unless the text below allows it;
+ *     elements of an output must not coincide, and an output must not overlap an input or another output unless the text below
+ *     allows it.  Column ranges of one buffer do not overlap if the tensors have the same row stride; tensors interleaved in some
+ *     other way are refused, since that cannot be told from an overlap;
  *   - any alignment of the element type is taken; rows that start on 16-byte boundaries are fastest;
  *   - the kernels are enqueued on `stream` (a cudaStream_t of the current device, NULL = its default stream) and the call
  *     returns without waiting.  Calls may be captured into a graph, and made from several threads at once on different buffers;
@@ -205,7 +207,7 @@ typedef struct kb_view {
  *   x [m][k], rows ldx apart      w [n][k], rows ldw apart (the order of a tensor-core convolution's weights, outC x inC)
  *   bias [n] fp32 or NULL         residual [m][n], rows ldr apart, or NULL
  *   y [m][n], rows ldy apart      act a KB_ACT_* of kb_modelblob.h
- * The residual may be y itself (same address, same stride).  m may be 0. */
+ * The residual may be y itself (same address, same stride).  m may be 0; m, n and k are at most 2^30. */
 int kb_matmul(
   int precision, int m, int n, int k, const void* x, int64_t ldx, const void* w, int64_t ldw, const float* bias, int act,
   const void* residual, int64_t ldr, void* y, int64_t ldy, void* stream);

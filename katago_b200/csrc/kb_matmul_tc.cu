@@ -439,6 +439,7 @@ __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
 }
 
 bool encodeRows(CUtensorMap* map, int dt, const void* p, int64_t cols, int64_t rows, int64_t ld, int boxCols, int boxRows, CUtensorMapSwizzle sw) {
+  if(rows == 1) ld = (cols + 7) / 8 * 8;  // nothing lies that far on
   const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)ld * 2};
   const uint32_t box[2] = {(uint32_t)boxCols, (uint32_t)boxRows};
   return encodeTiled(map, dt, p, 2, dims, strides, box, sw);

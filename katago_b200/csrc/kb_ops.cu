@@ -3,6 +3,7 @@
 #include "kb_ops.h"
 
 #include <cuda.h>
+#include <algorithm>
 #include <mutex>
 #include <stdexcept>
 #include <string>
@@ -88,10 +89,12 @@ bool mayOverlap(const Box& a, const Box& b) {
   if(a.empty() || b.empty()) return false;
   const int64_t pa = (int64_t)(uintptr_t)a.p, pb = (int64_t)(uintptr_t)b.p;
   if(pa + a.bytes() <= pb || pb + b.bytes() <= pa) return false;
-  // the same row stride (and batches of whole rows): compare the windows that each takes of a row
-  const int64_t row = a.s[1] * (int64_t)a.elem;
-  if(row <= 0 || row != b.s[1] * (int64_t)b.elem) return true;
-  if((a.n[0] > 1 && a.s[0] % a.s[1] != 0) || (b.n[0] > 1 && b.s[0] % b.s[1] != 0)) return true;
+  // rows of the same stride (tokens, or sequences of one token; batches of whole rows): compare the windows that each takes of a row
+  auto rowOf = [](const Box& x) { return (x.n[1] > 1 ? x.s[1] : (x.n[0] > 1 ? x.s[0] : 0)) * (int64_t)x.elem; };
+  const int64_t ra = rowOf(a), rb = rowOf(b), row = std::max(ra, rb);
+  if(row <= 0 || (ra != 0 && ra != row) || (rb != 0 && rb != row)) return true;
+  auto whole = [](const Box& x) { return x.n[0] == 1 || x.n[1] == 1 || x.s[0] % x.s[1] == 0; };
+  if(!whole(a) || !whole(b)) return true;
   const int64_t wa = ((a.n[2] - 1) * a.s[2] + a.width) * (int64_t)a.elem, wb = ((b.n[2] - 1) * b.s[2] + b.width) * (int64_t)b.elem;
   if(wa > row || wb > row) return true;
   const int64_t delta = (((pb - pa) % row) + row) % row;
@@ -187,9 +190,10 @@ void opMatmul(const MatmulArgs& given, void* stream) {
   const char* op = "kb_matmul";
   MatmulArgs a = given;
   const size_t es = elementSize(a.dt, op);
-  checkCount(op, "m", a.M, 0, INT32_MAX);
-  checkCount(op, "n", a.N, 1, INT32_MAX - 1024);
-  checkCount(op, "k", a.K, 1, INT32_MAX - 1024);
+  constexpr int64_t MOST = int64_t(1) << 30;
+  checkCount(op, "m", a.M, 0, MOST);
+  checkCount(op, "n", a.N, 1, MOST);
+  checkCount(op, "k", a.K, 1, MOST);
   if(a.act != KB_ACT_IDENTITY && a.act != KB_ACT_RELU && a.act != KB_ACT_MISH && a.act != KB_ACT_SILU && a.act != KB_ACT_MISH_SCALE8)
     refuse("kb_matmul: unknown activation " + std::to_string(a.act));
   if(a.ldx < a.K || a.ldw < a.K) refuse("kb_matmul: a row stride of x or w is smaller than k");

@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const R
   extern __shared__ unsigned long long sTurn[];  // [freqHeads][pairs][axes], or nothing
   gridDepLaunch();
   gridDepWait();
-  const int entries = a.freqHeads * (a.rot / 2) * a.axes;
+  const long long entries = (long long)a.freqHeads * (a.rot / 2) * a.axes;
   const bool table = entries <= ROPE_TABLE;
   if(table) {
     // the conversion of a frequency takes some ten fp64 operations: once per block, not once per token
@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const R
     const int32_t* pos = a.positions + b * a.posB + (long long)t * a.axes;
     auto angles = [&](int th) {
       have = th;
-      const int first = (th * pairs + c * P) * a.axes;
+      const long long first = ((long long)th * pairs + c * P) * a.axes;
       unsigned long long turn[P];
       bool finite[P];
 #pragma unroll
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const R
     auto tableOf = [&](int h) {
       return a.freqHeads == 1 ? 0 : (h < a.q.heads ? h / (a.q.heads / a.freqHeads) : (h - a.q.heads) / (a.k.heads / a.freqHeads));
     };
-    constexpr int U = 4;  // heads whose loads are in flight together
+    constexpr int U = MODE == 1 ? 3 : 4;  // heads whose loads are in flight together
     for(int hb = h0; hb < h1; hb += U) {
       constexpr int NV = MODE == 1 ? 1 : 2;
       constexpr int W = MODE == 0 ? 1 : V;
@@ -180,16 +180,16 @@ template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a)
   const int groups = (int)std::min<long long>(heads, std::max<long long>(1, want / perHead));
   const int headsPerItem = (heads + groups - 1) / groups;
   const long long items = perHead * ((heads + headsPerItem - 1) / headsPerItem);
-  const int entries = a.freqHeads * (a.rot / 2) * a.axes;
+  const long long entries = (long long)a.freqHeads * (a.rot / 2) * a.axes;
   const size_t smem = entries <= ROPE_TABLE ? (size_t)entries * 8 : 0;
   // Few blocks walk over the items, so that each converts the frequencies once.  Of 2 to 64 blocks per SM six were best: 128 x 361
-  // tokens of 12 heads of 64 (fp16, 142 MB) 28.2 us, 36 us with as many as are resident.  So were four resident blocks for
-  // adjacent pairs (34.7 us with two) and two for halves, which need their registers (2 x 20 280 tokens of 32 heads of 128, bf16,
-  // 664 MB: 124 us, 5.4 TB/s; 303 us with three, spilled).
+  // tokens of 12 heads of 64 (fp16, 142 MB) 29.8 us, 31.4 us with as many as are resident.  So were four resident blocks for
+  // adjacent pairs with three heads in flight (33 us with three blocks) and two for halves, which need their registers (2 x 20 280 tokens of 32
+  // heads of 128, bf16, 664 MB: 120 us, 5.5 TB/s; 303 us with three, spilled).
   const long long blocks = std::min<long long>((items + 255) / 256, 6LL * smCount());
   const dim3 grid((unsigned)blocks), block(256);
   auto run = [&](auto kernel) { return launchDependent(kernel, grid, block, smem, st, a, chunks, copies, headsPerItem, items); };
-  // (without channels to copy, a kernel without that loop: it costs the other one registers, 128 x 361 tokens 27.7 -> 32 us)
+  // (without channels to copy, a kernel without that loop: it costs the other one registers, 128 x 361 tokens 30 -> 32 us)
   if(!vec) return copies ? run(ropeAxesKernel<T, 0, 1, true>) : run(ropeAxesKernel<T, 0, 1, false>);
   if(a.halves) return copies ? run(ropeAxesKernel<T, 2, V, true>) : run(ropeAxesKernel<T, 2, V, false>);
   return copies ? run(ropeAxesKernel<T, 1, V, true>) : run(ropeAxesKernel<T, 1, V, false>);

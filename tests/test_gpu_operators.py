@@ -89,6 +89,19 @@ def test_matmul_rows_in_wider_buffers(dtype, m, shift):
 
 
 @pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("m", (1, 5, 30, 200, 3000))
+@pytest.mark.parametrize("n,k", [(70, 33), (130, 85), (264, 1301)])
+def test_matmul_odd_sums_in_aligned_rows(dtype, m, n, k):
+    """Rows on 16-byte boundaries whose last vector is cut: what lies behind it (NaN) is not summed."""
+    g = seeded(dtype, m, n, k)
+    ld = (k + 7) // 8 * 8 + 16
+    x, w = (torch.full((rows, ld), NAN, dtype=TYPES[dtype], device="cuda")[:, 8:8 + k] for rows in (m, n))
+    x.copy_(normal(g, m, k, dtype=dtype)), w.copy_(normal(g, n, k, dtype=dtype, scale=k ** -0.5))
+    want, bound = matmul_reference(dtype, x, w, None, 3, None)
+    assert_within(multiply(dtype, x, w, None, 3), want, bound)
+
+
+@pytest.mark.parametrize("dtype", ALL)
 @pytest.mark.parametrize("m,n,k", [(4, 200, 96), (40, 96, 512), (600, 512, 128), (33, 17, 9)])
 def test_matmul_adds_to_its_own_output(dtype, m, n, k):
     g = seeded(dtype, m, n)
@@ -201,6 +214,37 @@ def test_rope_in_place_on_a_merged_projection():
     assert_within(q, *want[0])
     assert_within(k, *want[1])
     assert torch.equal(whole[..., 256:], before[..., 256:])
+
+
+def test_rope_in_place_of_single_tokens_in_one_buffer():
+    """The newest token of each sequence: q and k side by side, whatever stride the only token has."""
+    g = seeded(2)
+    whole = normal(g, 5, 3 * 64, dtype="bf16")
+    before = whole.clone()
+    positions, freqs = angles_for(g, 5, 1, 1, 1, 16, 1 << 20)
+    q, k = (before[:, i:i + 64].reshape(5, 1, 2, 32) for i in (0, 64))
+    want = [rope_reference("bf16", x, positions, freqs, 32, True) for x in (q, k)]
+    v = [capi.View(whole.data_ptr() + 2 * 64 * i, 192, 0, 32) for i in (0, 1)]
+    capi.rope(PRECISION["bf16"], 5, 1, 32, 32, positions.data_ptr(), 1, 1, freqs.data_ptr(), 1, 1, v[0], v[0], 2, v[1], v[1], 2, stream())
+    for i in (0, 1):
+        assert_within(whole[:, 64 * i:64 * i + 64].reshape(5, 1, 2, 32), *want[i])
+    assert torch.equal(whole[:, 128:], before[:, 128:])
+
+
+@pytest.mark.parametrize("tables", (64, 4096))
+def test_rope_many_tables(tables):
+    """More frequencies than a block keeps: they are converted where they are used."""
+    g = seeded(tables)
+    heads = tables
+    q = normal(g, 1, 3, heads, 16, dtype="fp16")
+    positions, freqs = angles_for(g, 1, 3, 9, tables, 8, 1000)
+    freqs[1, 2, 4] = float("nan")
+    got, _ = turn("fp16", q, None, positions, freqs, 16, True)
+    want, bound = rope_reference("fp16", q, positions, freqs.nan_to_num(0.0), 16, True)
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[:, :, 1, 2] = bad[:, :, 1, 10] = True
+    assert got[bad].isnan().all()
+    assert_within(torch.where(bad, 0, got), torch.where(bad, 0, want), bound)
 
 
 def test_rope_of_an_infinite_frequency_is_nan_and_stays_in_its_pair():

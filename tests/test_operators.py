@@ -14,7 +14,7 @@ def matmul(precision=FP32, m=4, n=4, k=4, ldx=4, ldw=4, ldy=4, act=0, residual=0
 
 
 @pytest.mark.parametrize("given,says", [
-    (dict(precision=7), "unknown precision"), (dict(m=-1), "m is -1"), (dict(n=0), "n is 0"), (dict(k=0), "k is 0"), (dict(act=4), "unknown activation"),
+    (dict(precision=7), "unknown precision"), (dict(m=-1), "m is -1"), (dict(k=(1 << 30) + 1, ldx=1 << 31, ldw=1 << 31), "k is 1073741825"), (dict(n=2 ** 31 - 1), "n is 2147483647"), (dict(n=0), "n is 0"), (dict(k=0), "k is 0"), (dict(act=4), "unknown activation"),
     (dict(ldx=3), "row stride of x or w"), (dict(ldw=3), "row stride of x or w"), (dict(ldy=3), "row stride of y"), (dict(residual=P, ldr=3), "row stride of y or the residual"),
 ])
 def test_matmul_refuses(given, says):
