@@ -23,7 +23,7 @@ namespace {
 constexpr int XS_KEYS = 64, XS_THREADS = 256;
 
 __host__ __device__ constexpr int xsPitch(int d) { return (d + 3) / 4 * 4 + 4; }
-size_t xsSmem(int rows, int dq, int dv) { return sizeof(float) * (size_t)((rows + XS_KEYS) * xsPitch(dq) + XS_KEYS * xsPitch(dv) + rows * (XS_KEYS + 4)) + XS_KEYS; }
+size_t xsSmem(int rows, int dq, int dv) { return sizeof(float) * (size_t)((rows + XS_KEYS) * xsPitch(dq) + XS_KEYS * xsPitch(dv) + rows * (XS_KEYS + 4)) + 2 * XS_KEYS; }
 
 // Copies ROWS rows of d channels to fp32 rows of `pitch` in shared memory, zeros behind the last channel and for rows that
 // `row` gives no address for.  Eight lanes per row and four channels per lane, with several rows' loads in flight.
@@ -62,6 +62,21 @@ template <typename T, int ROWS, bool VEC, class Row> __device__ __forceinline__ 
   }
 }
 
+// The same without registers in between, for fp32 rows of whole vectors: asynchronous copies, zeros for rows without an address.
+template <int ROWS, class Row> __device__ __forceinline__ void xsStageAsync(float* dst, int pitch, const float* anywhere, Row row) {
+  const int lane8 = threadIdx.x & 7;
+#pragma unroll
+  for(int p = 0; p < (ROWS + XS_THREADS / 8 - 1) / (XS_THREADS / 8); p++) {
+    const int r = (threadIdx.x >> 3) + p * (XS_THREADS / 8);
+    if(r >= ROWS) break;
+    const float* from = row(r);
+    for(int c = lane8 * 4; c < pitch - 4; c += 32)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smemU32(dst + r * pitch + c)), "l"(from ? from + c : anywhere), "r"(from ? 16 : 0) : "memory");
+  }
+}
+__device__ __forceinline__ void xsCommit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void xsWaitAllButOne() { asm volatile("cp.async.wait_group 1;" ::: "memory"); }
+
 // NC: groups of 64 output channels; RI: rows per thread (16 threads share a row); VEC: channels in vectors of four
 template <typename T, int NC, int RI, bool VEC>
 __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 ? 2 : 1)) : (NC <= 2 ? 2 : 1)) crossAttnSimtKernel(const CrossAttnArgs a, const XaSplit sp) {
@@ -73,7 +88,8 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
   float* sK = sQ + ROWS * pq;
   float* sV = sK + XS_KEYS * pq;
   float* sP = sV + XS_KEYS * pv;
-  uint8_t* sOk = reinterpret_cast<uint8_t*>(sP + ROWS * PP);
+  uint8_t* sOk = reinterpret_cast<uint8_t*>(sP + ROWS * PP);  // [2]: of this tile of keys, of the next
+  constexpr bool ASYNC = VEC && sizeof(T) == 4;  // K of the next tile travels under this one's softmax and second product, V under the first
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
   const int CG = NC > 1 || a.dv > 32 ? 16 : (a.dv > 16 ? 8 : (a.dv > 8 ? 4 : 2)), KS = 16 / CG;
   const int cg = tx & (CG - 1), ks = tx / CG;
@@ -87,10 +103,25 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
   const int k0 = blk.part * sp.chunk, k1 = (int)min((long long)keys, (long long)k0 + sp.chunk);
   if(sp.parts > 1 && k0 >= keys && blk.part > 0) return;  // a part without keys; part 0 always reports
 
-  xsStage<T, ROWS, VEC>(sQ, pq, a.dq, [&](int r) -> const T* {
+  const T* kBase = (const T*)a.k + blk.b * a.kB + blk.kvh * a.kH;
+  const T* vBase = (const T*)a.v + blk.b * a.vB + blk.kvh * a.vH;
+  auto attended = [&](int key) { return key < k1 && (!a.keyMask || a.keyMask[(int64_t)blk.b * a.kLen + key] != 0.0f); };
+  auto qRow = [&](int r) -> const T* {
     r += blk.row0;
     return r < rows ? (const T*)a.q + blk.b * a.qB + (r / G) * a.qT + (blk.kvh * G + r % G) * a.qH : nullptr;
-  });
+  };
+  auto requestK = [&](int kt, const uint8_t* on) { xsStageAsync<XS_KEYS>(sK, pq, (const float*)a.q, [&](int j) { return on[j] ? (const float*)(kBase + (kt + j) * a.kT) : nullptr; }); };
+  auto requestV = [&](int kt, const uint8_t* on) { xsStageAsync<XS_KEYS>(sV, pv, (const float*)a.q, [&](int j) { return on[j] ? (const float*)(vBase + (kt + j) * a.vT) : nullptr; }); };
+  if(ASYNC) {
+    if(tid < XS_KEYS) sOk[tid] = attended(k0 + tid);
+    xsStageAsync<ROWS>(sQ, pq, (const float*)a.q, [&](int r) { return (const float*)qRow(r); });
+    __syncthreads();
+    requestK(k0, sOk);
+    xsCommit();
+    requestV(k0, sOk);
+    xsCommit();
+  }
+  else xsStage<T, ROWS, VEC>(sQ, pq, a.dq, qRow);
   float mx[RI], sum[RI];
   float4 o[RI][NC];
 #pragma unroll
@@ -101,15 +132,21 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
     for(int c = 0; c < NC; c++) o[i][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   const float scale = a.scale * 1.4426950408889634f;
-  const T* kBase = (const T*)a.k + blk.b * a.kB + blk.kvh * a.kH;
-  const T* vBase = (const T*)a.v + blk.b * a.vB + blk.kvh * a.vH;
   for(int kt = k0; kt < k1; kt += XS_KEYS) {
-    __syncthreads();
-    if(tid < XS_KEYS) sOk[tid] = kt + tid < k1 && (!a.keyMask || a.keyMask[(int64_t)blk.b * a.kLen + kt + tid] != 0.0f);
-    __syncthreads();
-    xsStage<T, XS_KEYS, VEC>(sK, pq, a.dq, [&](int j) { return sOk[j] ? kBase + (kt + j) * a.kT : nullptr; });
-    xsStage<T, XS_KEYS, VEC>(sV, pv, a.dv, [&](int j) { return sOk[j] ? vBase + (kt + j) * a.vT : nullptr; });
-    __syncthreads();
+    const uint8_t* on = sOk + (ASYNC ? ((kt - k0) / XS_KEYS & 1) * XS_KEYS : 0);
+    uint8_t* onNext = sOk + (ASYNC ? XS_KEYS - (on - sOk) : 0);
+    if(ASYNC) {
+      xsWaitAllButOne();  // K (and Q)
+      __syncthreads();
+    }
+    else {
+      __syncthreads();
+      if(tid < XS_KEYS) sOk[tid] = attended(kt + tid);
+      __syncthreads();
+      xsStage<T, XS_KEYS, VEC>(sK, pq, a.dq, [&](int j) { return on[j] ? kBase + (kt + j) * a.kT : nullptr; });
+      xsStage<T, XS_KEYS, VEC>(sV, pv, a.dv, [&](int j) { return on[j] ? vBase + (kt + j) * a.vT : nullptr; });
+      __syncthreads();
+    }
     // even and odd channels apart: the packed fp32 instructions do two IEEE operations per issue slot
     float2 s2[RI][4];
 #pragma unroll
@@ -136,12 +173,18 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
     for(int i = 0; i < RI; i++)
 #pragma unroll
       for(int j = 0; j < 4; j++) s[i][j] = s2[i][j].x + s2[i][j].y;
+    if(ASYNC) {
+      if(tid < XS_KEYS) onNext[tid] = attended(kt + XS_KEYS + tid);
+      __syncthreads();  // K has been read
+      if(kt + XS_KEYS < k1) requestK(kt + XS_KEYS, onNext);
+      xsCommit();
+    }
 #pragma unroll
     for(int i = 0; i < RI; i++) {
       float top = -INFINITY;
 #pragma unroll
       for(int j = 0; j < 4; j++) {
-        s[i][j] = sOk[tx + 16 * j] ? s[i][j] * scale : -INFINITY;
+        s[i][j] = on[tx + 16 * j] ? s[i][j] * scale : -INFINITY;
         top = fmaxf(top, s[i][j]);
       }
 #pragma unroll
@@ -161,6 +204,7 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
 #pragma unroll
       for(int c = 0; c < NC; c++) { o[i][c].x *= keep; o[i][c].y *= keep; o[i][c].z *= keep; o[i][c].w *= keep; }
     }
+    if(ASYNC) xsWaitAllButOne();  // V
     __syncthreads();
     // Output channels: CG threads have four each (of every 64 where there are more); the other threads of a row share the keys.
     for(int j = ks * 4; j < XS_KEYS; j += 4 * KS) {
@@ -187,7 +231,13 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
         }
       }
     }
+    if(ASYNC) {
+      __syncthreads();  // V has been read
+      if(kt + XS_KEYS < k1) requestV(kt + XS_KEYS, onNext);
+      xsCommit();
+    }
   }
+  if(ASYNC) asm volatile("cp.async.wait_group 0;" ::: "memory");
   if(KS > 1)
 #pragma unroll
     for(int i = 0; i < RI; i++)
