@@ -1,12 +1,10 @@
-// y = act(x w^T + bias) + residual on a caller's own matrices, on the CUDA cores: fp32, and 16-bit matrices whose rows do not
-// start on the boundaries that TMA needs.  (16-bit matrices with aligned rows: kb_matmul_tc.cu.)
+// y = act(x w^T + bias) + residual on a caller's own matrices: fp32, and the kernels for few rows of any type.  (More rows of 16-bit
+// types: kb_matmul_tc.cu.)
 //
 // matmulF32Kernel    fp32: one tile of BM x BN outputs per block, slices of 32 channels through three stages of asynchronous copies
 //                    (16 bytes, or 4 where rows lie anywhere).  FMA-bound.  A thread reads four channels of a row at a time and
 //                    sums even and odd channels apart with the packed fp32 instructions (two IEEE operations per issue slot, no
 //                    operand has to be doubled); the two are added at the end.
-// matmulTileKernel   16-bit rows on other than 16-byte boundaries: the same tiles, converted to fp32 while they are staged; the next
-//                    slice travels through registers while this one is multiplied.
 // matmulFewKernel    up to eight rows: memory-bound, the weights are read once.  A block has four weight rows and cuts K
 //                    over its warps, whose sums are added in warp order.
 // matmulFewMmaKernel the same for up to 16 rows of 16-bit types and K up to 1024, where a launch's latency is what counts.
@@ -128,109 +126,6 @@ __global__ void __launch_bounds__(BM / TM * (BN / TN) * KG) matmulF32Kernel(cons
     for(int j = 0; j < TN; j++) {
       const int n = n0 + tx + TX * j;
       if(m < a.M && n < a.N) matmulStore<float>(a, m, n, acc[i][j].x + acc[i][j].y);
-    }
-  }
-}
-
-// V: elements of K per global access
-template <typename T, int BM, int BN, int V>
-__global__ void __launch_bounds__(256) matmulTileKernel(const MatmulArgs a) {
-  constexpr int BK = 16, TM = BM / 16, TN = BN / 16;
-  constexpr int PA = BM + 4, PB = BN + 4;  // pitches: rows of 16 bytes, transposed stores spread over the banks
-  __shared__ __align__(16) float sA[2][BK][PA], sB[2][BK][PB];
-  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int tilesN = (a.N + BN - 1) / BN;
-  const long long tile = blockIdx.x;
-  const int m0 = (int)(tile / tilesN) * BM, n0 = (int)(tile % tilesN) * BN;
-  constexpr int PER_ROW = BK / V;                  // accesses per staged row
-  constexpr int ROWS = 256 / PER_ROW;              // rows per pass
-  constexpr int NA = (BM + ROWS - 1) / ROWS, NB = (BN + ROWS - 1) / ROWS;
-  const int lk = (tid % PER_ROW) * V, lr = tid / PER_ROW;
-  OpVec<T, V> ra[NA], rb[NB];
-  gridDepLaunch();
-  gridDepWait();
-  auto fetch = [&](int k0) {
-#pragma unroll
-    for(int i = 0; i < NA; i++) {
-      const int r = lr + i * ROWS, m = m0 + r, k = k0 + lk;
-#pragma unroll
-      for(int e = 0; e < V; e++) ra[i].e[e] = OpType<T>::from(0.0f);
-      if(r < BM && m < a.M && k < a.K) ra[i].load((const T*)a.x + (int64_t)m * a.ldx + k);  // K is a multiple of V
-    }
-#pragma unroll
-    for(int i = 0; i < NB; i++) {
-      const int r = lr + i * ROWS, n = n0 + r, k = k0 + lk;
-#pragma unroll
-      for(int e = 0; e < V; e++) rb[i].e[e] = OpType<T>::from(0.0f);
-      if(r < BN && n < a.N && k < a.K) rb[i].load((const T*)a.w + (int64_t)n * a.ldw + k);
-    }
-  };
-  auto stage = [&](int s) {
-#pragma unroll
-    for(int i = 0; i < NA; i++)
-      if(lr + i * ROWS < BM)
-#pragma unroll
-        for(int e = 0; e < V; e++) sA[s][lk + e][lr + i * ROWS] = OpType<T>::to(ra[i].e[e]);
-#pragma unroll
-    for(int i = 0; i < NB; i++)
-      if(lr + i * ROWS < BN)
-#pragma unroll
-        for(int e = 0; e < V; e++) sB[s][lk + e][lr + i * ROWS] = OpType<T>::to(rb[i].e[e]);
-  };
-  // thread (ty, tx): rows ty*4.. of every 64 (or ty*TM..), columns tx*4.. of every 64, or tx, tx + 16, ...
-  constexpr int CM = TM >= 4 ? 4 : TM, CN = TN % 4 == 0 ? 4 : 1;
-  auto col = [&](int j) { return (j / CN) * 16 * CN + tx * CN + j % CN; };
-  float2 acc[TM / 2][TN];  // pairs of rows
-#pragma unroll
-  for(int i = 0; i < TM / 2; i++)
-#pragma unroll
-    for(int j = 0; j < TN; j++) acc[i][j] = make_float2(0.0f, 0.0f);
-  const int steps = (a.K + BK - 1) / BK;
-  fetch(0);
-  stage(0);
-  __syncthreads();
-  for(int s = 0; s < steps; s++) {
-    if(s + 1 < steps) fetch((s + 1) * BK);
-    const int cur = s & 1;
-#pragma unroll
-    for(int k = 0; k < BK; k++) {
-      float2 av[TM / 2];
-      float bv[TN];
-#pragma unroll
-      for(int i = 0; i < TM / CM; i++) {
-        const float* p = &sA[cur][k][i * 16 * CM + ty * CM];
-        if(CM == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p);
-          av[i * 2] = make_float2(v.x, v.y);
-          av[(i * 2 + 1) % (TM / 2)] = make_float2(v.z, v.w);
-        }
-        else av[i] = *reinterpret_cast<const float2*>(p);
-      }
-#pragma unroll
-      for(int j = 0; j < TN / CN; j++) {
-        const float* p = &sB[cur][k][j * 16 * CN + tx * CN];
-        if(CN == 4) {
-          const float4 v = *reinterpret_cast<const float4*>(p);
-          bv[j * CN] = v.x; bv[(j * CN + 1) % TN] = v.y; bv[(j * CN + 2) % TN] = v.z; bv[(j * CN + 3) % TN] = v.w;
-        }
-        else bv[j] = *p;
-      }
-#pragma unroll
-      for(int i = 0; i < TM / 2; i++)
-#pragma unroll
-        for(int j = 0; j < TN; j++) acc[i][j] = __ffma2_rn(av[i], make_float2(bv[j], bv[j]), acc[i][j]);
-    }
-    if(s + 1 < steps) stage(cur ^ 1);
-    __syncthreads();
-  }
-#pragma unroll
-  for(int i = 0; i < TM; i++) {
-    const int m = m0 + (i / CM) * 16 * CM + ty * CM + i % CM;
-    if(m >= a.M) continue;
-#pragma unroll
-    for(int j = 0; j < TN; j++) {
-      const int n = n0 + col(j);
-      if(n < a.N) matmulStore<T>(a, m, n, i % 2 == 0 ? acc[i / 2][j].x : acc[i / 2][j].y);
     }
   }
 }
@@ -380,16 +275,7 @@ template <int N> cudaError_t launchTiles(cudaStream_t st, const MatmulArgs& a, c
   }
   return launchDependent(forms[pick].run, dim3((unsigned)count), dim3(forms[pick].threads), bytes, st, a);
 }
-template <typename T, int V> struct TileForms {
-  static cudaError_t launch(cudaStream_t st, const MatmulArgs& a) {
-    constexpr int VT = V > 4 ? 4 : V;  // elements of an access: four threads per staged row
-    static const TileForm forms[] = {{128, 128, 1.0, matmulTileKernel<T, 128, 128, VT>, 256, 0}, {64, 64, 1.25, matmulTileKernel<T, 64, 64, VT>, 256, 0},
-                                     {64, 48, 1.3, matmulTileKernel<T, 64, 48, VT>, 256, 0}, {32, 32, 2.0, matmulTileKernel<T, 32, 32, VT>, 256, 0}};
-    static SharedMemoryOptIn optIn[4];
-    return launchTiles(st, a, forms, optIn);
-  }
-};
-template <int V> struct TileForms<float, V> {
+template <int V> struct F32Forms {
   static cudaError_t launch(cudaStream_t st, const MatmulArgs& a) {
     static const TileForm forms[] = {form<128, 128, 8, 8, 1>(1.0), form<128, 64, 8, 8, 2>(1.1), form<64, 64, 8, 8, 4>(1.35), form<64, 48, 8, 6, 4>(1.4), form<32, 32, 4, 4, 4>(2.0)};
     static SharedMemoryOptIn optIn[5];
@@ -409,7 +295,8 @@ template <typename T, int V> cudaError_t matmulLaunch(cudaStream_t st, const Mat
     if(a.M <= 4) return launchDependent(matmulFewKernel<T, 4, V>, grid, block, 0, st, a);
     return launchDependent(matmulFewKernel<T, 8, V>, grid, block, 0, st, a);
   }
-  return TileForms<T, V>::launch(st, a);
+  if constexpr(std::is_same<T, float>::value) return F32Forms<V>::launch(st, a);
+  return cudaErrorInvalidValue;  // more tiles than a launch has blocks
 }
 
 template <typename T> cudaError_t matmulLaunchT(cudaStream_t st, const MatmulArgs& a) {
@@ -422,8 +309,9 @@ template <typename T> cudaError_t matmulLaunchT(cudaStream_t st, const MatmulArg
 
 cudaError_t launchMatmul(cudaStream_t st, const MatmulArgs& a) {
   if(matmulTcEligible(a)) {
-    if(a.M <= 16 && a.K % 8 == 0 && a.K <= 1024 && a.N <= 8192) return a.dt == DT_F16 ? matmulFewMma<__half>(st, a) : matmulFewMma<__nv_bfloat16>(st, a);
-    return launchMatmulTc(st, a);
+    const bool aligned = matmulTcAligned(a);
+    if(aligned && a.M <= 16 && a.K % 8 == 0 && a.K <= 1024 && a.N <= 8192) return a.dt == DT_F16 ? matmulFewMma<__half>(st, a) : matmulFewMma<__nv_bfloat16>(st, a);
+    if(aligned || a.M > 8) return launchMatmulTc(st, a);
   }
   switch(a.dt) {
     case DT_F32: return matmulLaunchT<float>(st, a);

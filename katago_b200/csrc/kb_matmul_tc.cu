@@ -8,6 +8,10 @@
 // residual and writes the slot's rows itself, a row per instruction.  (Eight warps, 32 or 64 columns at a time: 46208 x 1024 x 384
 // fp16 66 us with bias and SiLU; a warp's own chain of waits and special functions was what took the time.)
 //
+// Rows on other boundaries (PLAIN): eight warps take the place of TMA.  A warp reads a row's slice of 64 channels with two 2-byte loads per
+// lane, packs the pairs and writes the swizzled 128 bytes that TMA would have; sixteen rows are in flight.  The loads' latency
+// bounds it: 4097^3 bf16 1.25 ms, 110 TFLOP/s (4.2 ms where each load waited for the one before).  Eight warps then take accumulators out.
+//
 // matmulSkinnyKernel (few tiles): the weights are the 128 rows of a tile and up to 256 rows of x its columns, so that few rows of x
 // waste none of the tensor pipe and the weights are what streams.  A cluster of up to eight CTAs cuts K; each leaves its sums in its
 // own shared memory, and after a cluster barrier each adds a share of the rows of x over the cluster, in the order of K, through
@@ -28,7 +32,7 @@ namespace kb {
 namespace {
 
 constexpr int MT_BM = 128, MT_BK = 64, MT_UNIT = 32;  // rows, channels of a slice; columns of an output unit (of 32 rows)
-constexpr int MT_EPI_WARPS = 16, MT_GROUPS = MT_EPI_WARPS / 4, MT_THREADS = 64 + 32 * MT_EPI_WARPS;
+constexpr int MT_THREADS = 576, MT_LOADERS = 8;       // warps: request, multiply, sixteen for the output; or eight and MT_LOADERS
 constexpr int MT_A_BYTES = MT_BM * MT_BK * 2, MT_UNIT_BYTES = 32 * MT_UNIT * 2;
 constexpr int MT_MAX_STAGES = 8, MT_BAND = 16;
 constexpr int MT_ERR = 301;
@@ -48,10 +52,20 @@ __device__ __forceinline__ void mtTile(const MatmulTcArgs& a, int t, int& tm, in
   tm = band * MT_BAND + rest - tn * rows;
 }
 
-template <typename T>
+// Two neighbouring 16-bit elements at any address, each if its condition holds, else 0.  Predicated: a branch around each load would
+// wait for it.
+__device__ __forceinline__ void loadPair(const uint16_t* p, bool first, bool second, uint16_t& lo, uint16_t& hi) {
+  asm volatile(
+    "{\n\t.reg .pred a, b;\n\tsetp.ne.b32 a, %3, 0;\n\tsetp.ne.b32 b, %4, 0;\n\tmov.b16 %0, 0;\n\tmov.b16 %1, 0;\n\t"
+    "@a ld.global.b16 %0, [%2];\n\t@b ld.global.b16 %1, [%2+2];\n\t}"
+    : "=&h"(lo), "=&h"(hi) : "l"(p), "r"((int)first), "r"((int)second) : "memory");
+}
+
+template <typename T, bool PLAIN>
 __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
   const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
   const __grid_constant__ CUtensorMap tmR, const MatmulTcArgs a) {
+  constexpr int MT_EPI_WARPS = PLAIN ? 8 : 16, MT_GROUPS = MT_EPI_WARPS / 4;
   extern __shared__ uint8_t smemRaw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smemRaw) + 1023) & ~(uintptr_t)1023);
   const int slotBytes = MT_A_BYTES + a.BN * MT_BK * 2;
@@ -67,7 +81,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
 
   const int warp = warpIndex(), lane = threadIdx.x & 31;
   if(threadIdx.x == 0) {
-    for(int i = 0; i < MT_MAX_STAGES; i++) { mbarInit(smemU32(&bFull[i]), 1); mbarInit(smemU32(&bEmpty[i]), 1); }
+    for(int i = 0; i < MT_MAX_STAGES; i++) { mbarInit(smemU32(&bFull[i]), PLAIN ? MT_LOADERS : 1); mbarInit(smemU32(&bEmpty[i]), 1); }
     for(int i = 0; i < 2; i++) { mbarInit(smemU32(&bAcc[i]), 1); mbarInit(smemU32(&bTaken[i]), MT_EPI_WARPS); }
     for(int i = 0; i < MT_EPI_WARPS; i++) mbarInit(smemU32(&bRes[i]), 1);
     *abortFlag = 0;
@@ -75,7 +89,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
     fenceProxyAsync();
   }
   if(warp == 1) { tmemAlloc(smemU32(tmemSlot), a.tmemCols); tmemRelinquish(); }
-  if(warp == 0 && electOne()) { prefetchTensorMap(&tmX); prefetchTensorMap(&tmW); }
+  if(!PLAIN && warp == 0 && electOne()) { prefetchTensorMap(&tmX); prefetchTensorMap(&tmW); }
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
@@ -85,8 +99,46 @@ __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
   const int tiles = a.tilesM * a.tilesN;
   auto wait = [&](uint64_t* bar, uint32_t parity) { return opWait(smemU32(bar), parity, abortFlag, a.m.status, MT_ERR); };
 
-  if(warp == 0) {
-    if(electOne()) {
+  if(PLAIN && warp >= 2 + MT_EPI_WARPS) {
+    const int loader = warp - 2 - MT_EPI_WARPS;
+    const uint16_t* x = (const uint16_t*)a.m.x;
+    const uint16_t* w = (const uint16_t*)a.m.w;
+    uint32_t it = 0;
+    bool ok = true;
+    for(int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      int tm, tn;
+      mtTile(a, t, tm, tn);
+      for(int k = 0; k < a.kSlices; k++, it++) {
+        const uint32_t s = it % a.stages, use = it / a.stages;
+        if(use > 0) ok = wait(&bEmpty[s], (use - 1) & 1u);
+        if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+        uint8_t* slot = smem + (size_t)s * slotBytes;
+        const int c = k * MT_BK + 2 * lane;
+        constexpr int U = 16;
+        for(int r0 = loader; r0 < MT_BM + a.BN; r0 += MT_LOADERS * U) {
+          uint16_t lo[U], hi[U];
+#pragma unroll
+          for(int u = 0; u < U; u++) {
+            const int r = r0 + u * MT_LOADERS;  // rows of x, then rows of w
+            const bool isX = r < MT_BM;
+            const int row = isX ? tm * MT_BM + r : tn * a.BN + r - MT_BM;
+            const bool in = r < MT_BM + a.BN && row < (isX ? a.m.M : a.m.N);
+            loadPair((isX ? x + (int64_t)row * a.m.ldx : w + (int64_t)row * a.m.ldw) + c, in && c < a.m.K, in && c + 1 < a.m.K, lo[u], hi[u]);
+          }
+#pragma unroll
+          for(int u = 0; u < U; u++) {
+            const int r = r0 + u * MT_LOADERS;
+            if(r < MT_BM + a.BN) *reinterpret_cast<uint32_t*>(slot + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = lo[u] | (uint32_t)hi[u] << 16;
+          }
+        }
+        fenceProxyAsync();
+        __syncwarp();
+        if(lane == 0) mbarArrive(smemU32(&bFull[s]));
+      }
+    }
+  }
+  else if(warp == 0) {
+    if(!PLAIN && electOne()) {
       uint32_t it = 0;  // slices requested
       bool ok = true;
       for(int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
@@ -447,7 +499,7 @@ bool encodeRows(CUtensorMap* map, int dt, const void* p, int64_t cols, int64_t r
 
 bool rowsAligned(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
-template <typename T> cudaError_t launchWide(cudaStream_t st, const MatmulArgs& m) {
+template <typename T, bool PLAIN> cudaError_t launchWide(cudaStream_t st, const MatmulArgs& m) {
   MatmulTcArgs a = {};
   a.m = m;
   const int sms = smCount();
@@ -457,7 +509,7 @@ template <typename T> cudaError_t launchWide(cudaStream_t st, const MatmulArgs& 
   double best = 0;
   for(int bn = 256; bn >= 32; bn -= 32) {
     const double rounds = (double)(((long long)a.tilesM * ((m.N + bn - 1) / bn) + sms - 1) / sms);
-    const double cost = rounds * std::max({44.0, bn / 2.0, (MT_BM + bn) * 32 / 75.0});
+    const double cost = rounds * std::max({44.0, bn / 2.0, (MT_BM + bn) * 32 / (PLAIN ? 23.0 : 75.0)});
     if(a.BN == 0 || cost < best) { best = cost; a.BN = bn; }
   }
   a.tilesN = (m.N + a.BN - 1) / a.BN;
@@ -468,19 +520,19 @@ template <typename T> cudaError_t launchWide(cudaStream_t st, const MatmulArgs& 
   a.tmaOut = rowsAligned(m.y, m.ldy);
   a.tmaRes = a.tmaOut && m.residual && rowsAligned(m.residual, m.ldr);
   a.resAhead = a.tmaRes && a.kSlices < 16;  // ahead: a ring slot less for the products
-  const size_t fixed = MT_EPI_WARPS * (a.resAhead ? 2 : 1) * MT_UNIT_BYTES + 1024 + 512;
+  const size_t fixed = 16 * (a.resAhead ? 2 : 1) * MT_UNIT_BYTES + 1024 + 512;
   a.stages = (int)std::min<size_t>(MT_MAX_STAGES, (227 * 1024 - fixed) / slotBytes);
-  CUtensorMap x, w, y = {}, r = {};
-  bool ok = encodeRows(&x, m.dt, m.x, m.K, m.M, m.ldx, MT_BK, MT_BM, CU_TENSOR_MAP_SWIZZLE_128B) &&
-            encodeRows(&w, m.dt, m.w, m.K, m.N, m.ldw, MT_BK, a.BN, CU_TENSOR_MAP_SWIZZLE_128B);
+  CUtensorMap x = {}, w = {}, y = {}, r = {};
+  bool ok = PLAIN || (encodeRows(&x, m.dt, m.x, m.K, m.M, m.ldx, MT_BK, MT_BM, CU_TENSOR_MAP_SWIZZLE_128B) &&
+                      encodeRows(&w, m.dt, m.w, m.K, m.N, m.ldw, MT_BK, a.BN, CU_TENSOR_MAP_SWIZZLE_128B));
   if(a.tmaOut) ok = ok && encodeRows(&y, m.dt, m.y, m.N, m.M, m.ldy, MT_UNIT, 32, CU_TENSOR_MAP_SWIZZLE_64B);
   if(a.tmaRes) ok = ok && encodeRows(&r, m.dt, m.residual, m.N, m.M, m.ldr, MT_UNIT, 32, CU_TENSOR_MAP_SWIZZLE_64B);
   if(!ok) return cudaErrorInvalidValue;
   static SharedMemoryOptIn optIn;
-  const cudaError_t e = optIn((const void*)matmulTcKernel<T>, 227 * 1024);
+  const cudaError_t e = optIn((const void*)matmulTcKernel<T, PLAIN>, 227 * 1024);
   if(e != cudaSuccess) return e;
   const int tiles = a.tilesM * a.tilesN;
-  return launchDependent(matmulTcKernel<T>, dim3(std::min(tiles, sms)), dim3(MT_THREADS), (size_t)a.stages * slotBytes + fixed, st, x, w, y, r, a);
+  return launchDependent(matmulTcKernel<T, PLAIN>, dim3(std::min(tiles, sms)), dim3(MT_THREADS), (size_t)a.stages * slotBytes + fixed, st, x, w, y, r, a);
 }
 
 constexpr int MS_SMEM_TWO = 110 * 1024, MS_SMEM = 226 * 1024;  // of a CTA: two to an SM, one
@@ -540,15 +592,16 @@ template <typename T> cudaError_t launchSkinny(cudaStream_t st, MatmulSkinnyArgs
 }  // namespace
 
 bool matmulTcEligible(const MatmulArgs& a) {
-  return (a.dt == DT_F16 || a.dt == DT_BF16) && rowsAligned(a.x, a.ldx) && rowsAligned(a.w, a.ldw) &&
-         ((long long)a.M + 127) / 128 * (((long long)a.N + 31) / 32) < (1LL << 31);
+  return (a.dt == DT_F16 || a.dt == DT_BF16) && ((long long)a.M + 127) / 128 * (((long long)a.N + 31) / 32) < (1LL << 31);
 }
+bool matmulTcAligned(const MatmulArgs& a) { return rowsAligned(a.x, a.ldx) && rowsAligned(a.w, a.ldw); }
 
 cudaError_t launchMatmulTc(cudaStream_t st, const MatmulArgs& m) {
+  if(!matmulTcAligned(m)) return m.dt == DT_F16 ? launchWide<__half, true>(st, m) : launchWide<__nv_bfloat16, true>(st, m);
   MatmulSkinnyArgs a = {};
   a.m = m;
   if(skinnyShape(m, a)) return m.dt == DT_F16 ? launchSkinny<__half>(st, a) : launchSkinny<__nv_bfloat16>(st, a);
-  return m.dt == DT_F16 ? launchWide<__half>(st, m) : launchWide<__nv_bfloat16>(st, m);
+  return m.dt == DT_F16 ? launchWide<__half, false>(st, m) : launchWide<__nv_bfloat16, false>(st, m);
 }
 
 }  // namespace kb

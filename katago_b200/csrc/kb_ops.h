@@ -34,8 +34,9 @@ struct MatmulArgs {
   int* status;                 // receives the code of a device-side wait that ran out
 };
 cudaError_t launchMatmul(cudaStream_t st, const MatmulArgs& a);
-// kb_matmul_tc.cu: 16-bit types, rows of x and w on 16-byte boundaries
+// kb_matmul_tc.cu: 16-bit types; fastest with the rows of x and w on 16-byte boundaries
 bool matmulTcEligible(const MatmulArgs& a);
+bool matmulTcAligned(const MatmulArgs& a);
 cudaError_t launchMatmulTc(cudaStream_t st, const MatmulArgs& a);
 
 // ---- rotary positions ----
