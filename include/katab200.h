@@ -231,7 +231,7 @@ int kb_rope(
  *   q [batch][qLen][heads][qkDim]   k [batch][kLen][kvHeads][qkDim]   v [batch][kLen][kvHeads][vDim]
  *   out [batch][qLen][heads][vDim]  head sizes 1..256, heads a multiple of kvHeads, scale > 0
  *   qLengths, kLengths [batch] int32 on the device or NULL: rows of `out` from qLengths[b] on are left as they are; keys from
- *             kLengths[b] on are not read.  Values outside 0..qLen / 0..kLen count as the nearer end
+ *             kLengths[b] on are left out, whatever they hold.  Values outside 0..qLen / 0..kLen count as the nearer end
  *   keyMask   [batch][kLen] fp32 or NULL: keys whose mask is 0 are left out, whatever their k and v hold (NaN and Inf included)
  *   queryMask [batch][qLen] fp32 or NULL: tokens whose mask is 0 get a row of zeros
  * A row that no key is left for is zeros.

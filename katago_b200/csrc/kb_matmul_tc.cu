@@ -1,4 +1,4 @@
-// y = act(x w^T + bias) + residual on the tensor cores: fp16 / bf16 matrices whose rows start on 16-byte boundaries.
+// y = act(x w^T + bias) + residual on the tensor cores: fp16 / bf16.
 //
 // matmulTcKernel: persistent CTAs of 128 x BN tiles.  Warp 0 feeds 64-channel slices of x and w into a ring of slots by TMA
 // (128-byte swizzle; what a tile has beyond the matrices' ends is zero-filled), warp 1 issues tcgen05.mma into one of two
@@ -12,7 +12,7 @@
 // lane, packs the pairs and writes the swizzled 128 bytes that TMA would have; sixteen rows are in flight.  The loads' latency
 // bounds it: 4097^3 bf16 1.25 ms, 110 TFLOP/s (4.2 ms where each load waited for the one before).  Eight warps then take accumulators out.
 //
-// matmulSkinnyKernel (few tiles): the weights are the 128 rows of a tile and up to 256 rows of x its columns, so that few rows of x
+// matmulSkinnyKernel (few tiles): the weights are the 128 rows of a tile and up to 128 rows of x its columns, so that few rows of x
 // waste none of the tensor pipe and the weights are what streams.  A cluster of up to eight CTAs cuts K; each leaves its sums in its
 // own shared memory, and after a cluster barrier each adds a share of the rows of x over the cluster, in the order of K, through
 // distributed shared memory: no workspace, no second launch, the same order every time.

@@ -4,11 +4,13 @@
 // The rows of a key head are its query heads' rows side by side: row r = token r / G, head kvHead * G + r % G with G = heads /
 // kvHeads, so that grouped heads read K and V once.  A block takes 64 such rows (16 where there are no more) and a range of keys, 64 at a time: scores into
 // registers (4 x 4 or 1 x 4 per thread), a running maximum and sum per row, probabilities through shared memory, output accumulators in
-// registers.  All in fp32.  Keys behind a sequence's length are not read; masked keys' rows of K and V are replaced by zeros
-// while they are staged, so that nothing in them (NaN, Inf) reaches a product.
+// registers.  All in fp32.  Keys behind a sequence's length and masked keys are not read: their rows of K and V are zeros
+// in shared memory, so that nothing in them (NaN, Inf) reaches a product.  fp32 rows of whole vectors are copied asynchronously, the next
+// tile's under this one's products (16 x 361 tokens and states, 6 heads of 64: 117 us, 133 us through registers).
 //
 // A row's state is (maximum, sum, unnormalised output).  Where few rows have many keys the keys are cut into parts of `chunk`
-// keys, one block each; a part writes its state to the workspace and crossAttnJoinKernel adds the parts in order.
+// keys, one block each; a part writes its state to the workspace and crossAttnJoinKernel adds the parts in order (crossAttnJoinManyKernel
+// where there are many rows).
 #include "kb_kernels.cuh"
 #include "kb_ops.h"
 #include "kb_ops_dev.cuh"

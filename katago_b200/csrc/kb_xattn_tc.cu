@@ -5,9 +5,10 @@
 // time.  Two warpgroups do the softmax of one row tile each, a row per thread; of the third, warp 8 requests Q, K and V by TMA,
 // warp 9 issues the MMAs, warps 10 and 11 make the keys of a tile that are not attended harmless.
 //
-//   S = Q K^T into 128 columns of tensor memory, the probabilities (16 bit, two per column) back over the same columns, O = P V with P
-//   read from tensor memory into 64 or 128 further columns.  With two row tiles the tensor pipe works on one while the other's
-//   warpgroup does its exponentials:  S0(j) | PV1(j-1) | S1(j) | PV0(j) | S0(j+1) ...
+//   S = Q K^T into 128 columns of tensor memory, the probabilities (16 bit, two per column) back into tensor memory, O = P V with P
+//   read from there into 64 or 128 further columns.  With two row tiles the tensor pipe works on one while the other's warpgroup
+//   does its exponentials.  With head size 64 the probabilities have columns of their own, and a row tile's next scores are
+//   computed before its product; with 128 there is no room, they lie over the scores, and the next scores follow the product.
 //   A block with one row tile gives the warpgroups every other tile of keys instead, and adds the two states at the end.
 //
 // The row maximum is kept in units of log2; p = 2^(scale log2(e) s - ref), where ref follows the maximum only when that has grown by
