@@ -345,12 +345,6 @@ struct MatmulSkinnyArgs {
   uint32_t idesc, tmemCols;
 };
 
-__device__ __forceinline__ float4 ldCluster(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
   const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const MatmulSkinnyArgs a) {
@@ -467,7 +461,7 @@ __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
     else {
 #pragma unroll
       for(int s = 0; s < 8; s++)
-        if(s < a.split) p[s] = ldCluster(clusterMapAddr(mine + (uint32_t)r * (MT_BM * 4), (uint32_t)s));
+        if(s < a.split) p[s] = ldCluster4(clusterMapAddr(mine + (uint32_t)r * (MT_BM * 4), (uint32_t)s));
 #pragma unroll
       for(int s = 0; s < 8; s++)
         if(s < a.split) { v.x += p[s].x; v.y += p[s].y; v.z += p[s].z; v.w += p[s].w; }

@@ -55,6 +55,41 @@ template <typename T> __device__ __forceinline__ float opAct(float v, int act) {
   return applyActF(v, act);
 }
 
+// The same for several fp32 values: one choice of the function for all of them.
+template <int U> __device__ __forceinline__ void opActF32(float (&v)[U], int act) {
+  switch(act) {
+    case KB_ACT_RELU:
+#pragma unroll
+      for(int u = 0; u < U; u++) v[u] = applyActF(v[u], KB_ACT_RELU);
+      break;
+    case KB_ACT_SILU:
+#pragma unroll
+      for(int u = 0; u < U; u++) v[u] = applyActF(v[u], KB_ACT_SILU);
+      break;
+    case KB_ACT_MISH:
+#pragma unroll
+      for(int u = 0; u < U; u++) v[u] = opMish(v[u], v[u]);
+      break;
+    case KB_ACT_MISH_SCALE8:
+#pragma unroll
+      for(int u = 0; u < U; u++) v[u] = opMish(v[u], 8.0f * v[u]);
+      break;
+    default: break;
+  }
+}
+
+// Reads of another block's shared memory (an address that clusterMapAddr gave).
+__device__ __forceinline__ float4 ldCluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float ldCluster1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
 // Bounded wait of a role of these kernels (about 2 s).  A wait that runs out raises the abort flag and leaves `code` in the status
 // word, which is page-locked host memory (hence a plain store); it returns false, as does one that finds the flag raised, and
 // the role then leaves its loops.

@@ -59,6 +59,27 @@ def test_matmul_against_its_definition(dtype, m, n, k):
         assert_within(multiply(dtype, x, w, b, act, r), want, bound, f"act {act}")
 
 
+# fp32 sums that blocks of a cluster share (K in 1, 2, 4 and 8 parts, the last one shorter), rows on and off 16-byte boundaries,
+# tiles of each size with partial last ones, rows that are just too many for the kernel of few
+SHARED_SUMS = [(20, 64, 8000), (17, 35, 8193), (100, 100, 2500), (200, 132, 4100), (361, 513, 1030), (361, 512, 4096), (64, 388, 260), (1000, 1000, 900),
+               (1003, 1000, 2500), (1083, 364, 361), (2048, 700, 1100), (4001, 1201, 67), (4000, 1200, 33), (9, 4096, 4096), (16, 301, 2049), (12, 3001, 136), (17, 3001, 136)]
+
+
+@pytest.mark.parametrize("m,n,k", SHARED_SUMS)
+def test_matmul_shared_sums(m, n, k):
+    g = seeded(m, n, k)
+    x, w = normal(g, m, k, dtype="fp32"), normal(g, n, k, dtype="fp32", scale=k ** -0.5)
+    bias, residual = normal(g, n), normal(g, m, n, dtype="fp32")
+    want, bound = matmul_reference("fp32", x, w, bias, 2, residual)
+    y = residual.clone()
+    assert_within(multiply("fp32", x, w, bias, 2, y, y), want, bound, "adding to its own output")
+    assert torch.equal(multiply("fp32", x, w, bias, 2, residual), y), "the same sums every time"
+    want, bound = matmul_reference("fp32", x, w, None, 0, None)
+    wide = torch.full((m, n + 5), 7.0, device="cuda")  # rows of y off 16-byte boundaries, the columns behind them untouched
+    assert_within(multiply("fp32", x, w, y=wide[:, 1:1 + n]), want, bound, "rows in a wider buffer")
+    assert (wide[:, 0] == 7).all() and (wide[:, 1 + n:] == 7).all()
+
+
 @pytest.mark.parametrize("dtype", ALL)
 def test_matmul_every_activation(dtype):
     g = seeded(dtype)
