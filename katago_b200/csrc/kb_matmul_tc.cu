@@ -8,9 +8,10 @@
 // residual and writes the slot's rows itself, a row per instruction.  (Eight warps, 32 or 64 columns at a time: 46208 x 1024 x 384
 // fp16 66 us with bias and SiLU; a warp's own chain of waits and special functions was what took the time.)
 //
-// Rows on other boundaries (PLAIN): eight warps take the place of TMA.  A warp reads a row's slice of 64 channels with two 2-byte loads per
-// lane, packs the pairs and writes the swizzled 128 bytes that TMA would have; sixteen rows are in flight.  The loads' latency
-// bounds it: 4097^3 bf16 1.25 ms, 110 TFLOP/s (4.2 ms where each load waited for the one before).  Eight warps then take accumulators out.
+// Rows on other boundaries (PLAIN, both kernels): eight warps take the place of TMA and write the swizzled 128 bytes of a row that it would
+// have.  Rows on 4-byte boundaries go by asynchronous copies of two channels per lane (4096 x 4096 x 4098 bf16 860 us, 160 TFLOP/s;
+// the copies' rate bounds it), others by two 2-byte loads per lane with sixteen rows in flight, whose latency bounds it (4097^3 bf16
+// 1.30 ms, 105 TFLOP/s).  Eight warps then take accumulators out.
 //
 // matmulSkinnyKernel (few tiles): the weights are the 128 rows of a tile and up to 128 rows of x its columns, so that few rows of x
 // waste none of the tensor pipe and the weights are what streams.  A cluster of up to eight CTAs cuts K; each leaves its sums in its
@@ -61,6 +62,80 @@ __device__ __forceinline__ void loadPair(const uint16_t* p, bool first, bool sec
     : "=&h"(lo), "=&h"(hi) : "l"(p), "r"((int)first), "r"((int)second) : "memory");
 }
 
+// Rows of a matrix from `row0` on, `end` in all.
+struct PlainRows {
+  const uint16_t* p;
+  int64_t ld;
+  int row0, end;
+};
+
+// The slices of 64 channels that MT_LOADERS warps bring into the ring in place of TMA: 128 rows of `a`, then `nb` rows of `b`, each as
+// 128 bytes in the 128-byte swizzle; zeros beyond the ends.  Rows on 4-byte boundaries are copied asynchronously, two channels per lane, and a
+// slice is announced when those of the two after it have been requested; others go through registers, U rows in flight.
+template <int U, bool PAIRS> struct PlainLoader {
+  uint64_t* full;
+  int stages, K, loader, lane;
+  uint32_t it;  // slices requested
+
+  __device__ __forceinline__ uint32_t lag() const { return stages >= 3 ? 2u : 0u; }  // with fewer slots a wait for a free one would be for itself
+  __device__ __forceinline__ void announce(uint32_t i) {
+    fenceProxyAsync();
+    __syncwarp();
+    if(lane == 0) mbarArrive(smemU32(&full[i % (uint32_t)stages]));
+  }
+  __device__ __forceinline__ void slice(uint8_t* slot, const PlainRows& a, const PlainRows& b, int nb, int k) {
+    const int c = k * MT_BK + 2 * lane, rows = MT_BM + nb;
+    if(PAIRS) {
+      const uint32_t bytes = c + 1 < K ? 4 : c < K ? 2 : 0;
+#pragma unroll 4
+      for(int r = loader; r < rows; r += MT_LOADERS) {
+        const bool first = r < MT_BM;
+        const int row = first ? a.row0 + r : b.row0 + r - MT_BM;
+        const uint32_t n = row < (first ? a.end : b.end) ? bytes : 0u;
+        const uint16_t* src = first ? a.p + row * a.ld + c : b.p + row * b.ld + c;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smemU32(slot + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4)), "l"(n ? src : a.p), "r"(n) : "memory");
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if(lag() == 2) {
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+        if(it >= 2) announce(it - 2);
+      }
+      else {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        announce(it);
+      }
+    }
+    else {
+      for(int r0 = loader; r0 < rows; r0 += MT_LOADERS * U) {
+        uint16_t lo[U], hi[U];
+#pragma unroll
+        for(int u = 0; u < U; u++) {
+          const int r = r0 + u * MT_LOADERS;
+          const bool first = r < MT_BM;
+          const int row = first ? a.row0 + r : b.row0 + r - MT_BM;
+          const bool in = r < rows && row < (first ? a.end : b.end);
+          loadPair((first ? a.p + row * a.ld : b.p + row * b.ld) + c, in && c < K, in && c + 1 < K, lo[u], hi[u]);
+        }
+#pragma unroll
+        for(int u = 0; u < U; u++) {
+          const int r = r0 + u * MT_LOADERS;
+          if(r < rows) *reinterpret_cast<uint32_t*>(slot + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = lo[u] | (uint32_t)hi[u] << 16;
+        }
+      }
+      announce(it);
+    }
+    it++;
+  }
+  __device__ __forceinline__ void finish() {
+    if(!PAIRS) return;
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    for(uint32_t i = it > lag() ? it - lag() : 0; i < it; i++) announce(i);
+  }
+};
+
+// Whether rows start on 4-byte boundaries.
+__device__ __forceinline__ bool pairRows(const MatmulArgs& m) { return (((uintptr_t)m.x | (uintptr_t)m.w) & 3) == 0 && ((m.ldx | m.ldw) & 1) == 0; }
+
 template <typename T, bool PLAIN>
 __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
   const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmY,
@@ -101,41 +176,23 @@ __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
 
   if(PLAIN && warp >= 2 + MT_EPI_WARPS) {
     const int loader = warp - 2 - MT_EPI_WARPS;
-    const uint16_t* x = (const uint16_t*)a.m.x;
-    const uint16_t* w = (const uint16_t*)a.m.w;
-    uint32_t it = 0;
-    bool ok = true;
-    for(int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
-      int tm, tn;
-      mtTile(a, t, tm, tn);
-      for(int k = 0; k < a.kSlices; k++, it++) {
-        const uint32_t s = it % a.stages, use = it / a.stages;
-        if(use > 0) ok = wait(&bEmpty[s], (use - 1) & 1u);
-        if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
-        uint8_t* slot = smem + (size_t)s * slotBytes;
-        const int c = k * MT_BK + 2 * lane;
-        constexpr int U = 16;
-        for(int r0 = loader; r0 < MT_BM + a.BN; r0 += MT_LOADERS * U) {
-          uint16_t lo[U], hi[U];
-#pragma unroll
-          for(int u = 0; u < U; u++) {
-            const int r = r0 + u * MT_LOADERS;  // rows of x, then rows of w
-            const bool isX = r < MT_BM;
-            const int row = isX ? tm * MT_BM + r : tn * a.BN + r - MT_BM;
-            const bool in = r < MT_BM + a.BN && row < (isX ? a.m.M : a.m.N);
-            loadPair((isX ? x + (int64_t)row * a.m.ldx : w + (int64_t)row * a.m.ldw) + c, in && c < a.m.K, in && c + 1 < a.m.K, lo[u], hi[u]);
-          }
-#pragma unroll
-          for(int u = 0; u < U; u++) {
-            const int r = r0 + u * MT_LOADERS;
-            if(r < MT_BM + a.BN) *reinterpret_cast<uint32_t*>(slot + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = lo[u] | (uint32_t)hi[u] << 16;
-          }
+    auto run = [&](auto load) {
+      bool ok = true;
+      for(int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        int tm, tn;
+        mtTile(a, t, tm, tn);
+        const PlainRows x = {(const uint16_t*)a.m.x, a.m.ldx, tm * MT_BM, a.m.M}, w = {(const uint16_t*)a.m.w, a.m.ldw, tn * a.BN, a.m.N};
+        for(int k = 0; k < a.kSlices; k++) {
+          const uint32_t s = load.it % a.stages, use = load.it / a.stages;
+          if(use > 0) ok = wait(&bEmpty[s], (use - 1) & 1u);
+          if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+          load.slice(smem + (size_t)s * slotBytes, x, w, a.BN, k);
         }
-        fenceProxyAsync();
-        __syncwarp();
-        if(lane == 0) mbarArrive(smemU32(&bFull[s]));
       }
-    }
+      load.finish();
+    };
+    if(pairRows(a.m)) run(PlainLoader<16, true>{bFull, a.stages, a.m.K, loader, lane, 0});
+    else run(PlainLoader<16, false>{bFull, a.stages, a.m.K, loader, lane, 0});
   }
   else if(warp == 0) {
     if(!PLAIN && electOne()) {
@@ -345,7 +402,7 @@ struct MatmulSkinnyArgs {
   uint32_t idesc, tmemCols;
 };
 
-template <typename T>
+template <typename T, bool PLAIN>
 __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
   const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmW, const MatmulSkinnyArgs a) {
   extern __shared__ uint8_t smemRaw[];
@@ -357,14 +414,14 @@ __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
   volatile int* abortFlag = &abortWord;
   const int warp = warpIndex(), lane = threadIdx.x & 31;
   if(threadIdx.x == 0) {
-    for(int i = 0; i < a.stages; i++) { mbarInit(smemU32(&bFull[i]), 1); mbarInit(smemU32(&bEmpty[i]), 1); }
+    for(int i = 0; i < a.stages; i++) { mbarInit(smemU32(&bFull[i]), PLAIN ? MT_LOADERS : 1); mbarInit(smemU32(&bEmpty[i]), 1); }
     mbarInit(smemU32(&bAcc), 1);
     *abortFlag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     fenceProxyAsync();
   }
   if(warp == 1) { tmemAlloc(smemU32(&tmemSlot), a.tmemCols); tmemRelinquish(); }
-  if(warp == 0 && electOne()) { prefetchTensorMap(&tmX); prefetchTensorMap(&tmW); }
+  if(!PLAIN && warp == 0 && electOne()) { prefetchTensorMap(&tmX); prefetchTensorMap(&tmW); }
   tcFenceBefore();
   __syncthreads();
   tcFenceAfter();
@@ -377,8 +434,23 @@ __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
   const int s0 = (int)((long long)rank * a.kSlices / a.split), s1 = (int)((long long)(rank + 1) * a.kSlices / a.split);
   auto wait = [&](uint64_t* bar, uint32_t parity) { return opWait(smemU32(bar), parity, abortFlag, a.m.status, MS_ERR); };
 
-  if(warp == 0) {
-    if(electOne()) {
+  if(PLAIN && warp >= 2) {
+    auto run = [&](auto load) {
+      const PlainRows w = {(const uint16_t*)a.m.w, a.m.ldw, n0, a.m.N}, x = {(const uint16_t*)a.m.x, a.m.ldx, m0, a.m.M};
+      bool ok = true;
+      for(int k = s0; k < s1; k++) {
+        const uint32_t s = load.it % a.stages, use = load.it / a.stages;
+        if(use > 0) ok = wait(&bEmpty[s], (use - 1) & 1u);
+        if(__any_sync(0xffffffffu, !ok)) break;
+        load.slice(smem + (size_t)s * slotBytes, w, x, a.BN, k);
+      }
+      load.finish();
+    };
+    if(pairRows(a.m)) run(PlainLoader<8, true>{bFull, a.stages, a.m.K, warp - 2, lane, 0});
+    else run(PlainLoader<8, false>{bFull, a.stages, a.m.K, warp - 2, lane, 0});
+  }
+  else if(warp == 0) {
+    if(!PLAIN && electOne()) {
       uint32_t it = 0;
       bool ok = true;
       for(int k = s0; k < s1; k++, it++) {
@@ -533,8 +605,9 @@ constexpr int MS_SMEM_TWO = 110 * 1024, MS_SMEM = 226 * 1024;  // of a CTA: two 
 
 // Whether the skinny form runs these sizes, and how.  Up to 128 rows of x: always (4096 x 4096 bf16, 128 rows: 13.1 us, 20.2 us in wide
 // tiles).  More: where the wide tiles are one round at most and K is long enough to be worth cutting (300 x 512 x 4096: 8.5 us; but
-// 361 x 1024 x 384: 8.1 us against 4.5 us in 96 wide tiles).
-bool skinnyShape(const MatmulArgs& m, MatmulSkinnyArgs& a) {
+// 361 x 1024 x 384: 8.1 us against 4.5 us in 96 wide tiles).  Rows without TMA, whose slices take longer, are worth cutting earlier
+// (278 x 308 x 4706 bf16: 36 us, 213 us in wide tiles; 135 x 102 x 1442: 11 and 69; 16 x 181 x 236: 5.5 and 18).
+bool skinnyShape(const MatmulArgs& m, bool plain, MatmulSkinnyArgs& a) {
   const int sms = smCount();
   a.kSlices = (m.K + MT_BK - 1) / MT_BK;
   const int tilesW = (m.N + MT_BM - 1) / MT_BM;
@@ -542,25 +615,25 @@ bool skinnyShape(const MatmulArgs& m, MatmulSkinnyArgs& a) {
   a.BN = ((m.M + parts - 1) / parts + 15) / 16 * 16;
   a.tilesX = (m.M + a.BN - 1) / a.BN;
   const long long tiles = (long long)a.tilesX * tilesW;
-  if(m.M > 128 ? tiles > sms || a.kSlices < 32 : m.M > 16 && a.kSlices < 16) return false;
+  if(m.M > 128 ? tiles > sms || a.kSlices < (plain ? 8 : 32) : m.M > 16 && a.kSlices < (plain ? 4 : 16)) return false;
   a.split = 1;
-  while(a.split < 8 && tiles * a.split * 2 <= 2 * sms && a.split * 4 <= a.kSlices) a.split *= 2;
+  while(a.split < 8 && tiles * a.split * 2 <= 2 * sms && a.split * (plain ? 2 : 4) <= a.kSlices) a.split *= 2;
   return tiles * a.split < (1LL << 31);
 }
 
-template <typename T> cudaError_t launchSkinny(cudaStream_t st, MatmulSkinnyArgs a) {
+template <typename T, bool PLAIN> cudaError_t launchSkinny(cudaStream_t st, MatmulSkinnyArgs a) {
   const MatmulArgs& m = a.m;
   const int slotBytes = MT_A_BYTES + a.BN * MT_BK * 2, sumBytes = a.BN * MT_BM * 4;
   a.stages = std::min({MS_MAX_STAGES, ((sumBytes + 1024 <= MS_SMEM_TWO ? MS_SMEM_TWO : MS_SMEM) - 1024) / slotBytes, (a.kSlices + a.split - 1) / a.split});
   a.idesc = opIdesc<T>(MT_BM, a.BN);
   a.tmemCols = 32;
   while(a.tmemCols < (uint32_t)a.BN) a.tmemCols *= 2;
-  CUtensorMap x, w;
-  if(!encodeRows(&x, m.dt, m.x, m.K, m.M, m.ldx, MT_BK, a.BN, CU_TENSOR_MAP_SWIZZLE_128B) ||
-     !encodeRows(&w, m.dt, m.w, m.K, m.N, m.ldw, MT_BK, MT_BM, CU_TENSOR_MAP_SWIZZLE_128B))
+  CUtensorMap x = {}, w = {};
+  if(!PLAIN && (!encodeRows(&x, m.dt, m.x, m.K, m.M, m.ldx, MT_BK, a.BN, CU_TENSOR_MAP_SWIZZLE_128B) ||
+     !encodeRows(&w, m.dt, m.w, m.K, m.N, m.ldw, MT_BK, MT_BM, CU_TENSOR_MAP_SWIZZLE_128B)))
     return cudaErrorInvalidValue;
   static SharedMemoryOptIn optIn;
-  cudaError_t e = optIn((const void*)matmulSkinnyKernel<T>, MS_SMEM);
+  cudaError_t e = optIn((const void*)matmulSkinnyKernel<T, PLAIN>, MS_SMEM);
   if(e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.tilesX * ((m.N + MT_BM - 1) / MT_BM) * a.split));
@@ -580,7 +653,7 @@ template <typename T> cudaError_t launchSkinny(cudaStream_t st, MatmulSkinnyArgs
     n++;
   }
   cfg.attrs = attr; cfg.numAttrs = n;
-  return cudaLaunchKernelEx(&cfg, matmulSkinnyKernel<T>, x, w, a);
+  return cudaLaunchKernelEx(&cfg, matmulSkinnyKernel<T, PLAIN>, x, w, a);
 }
 
 }  // namespace
@@ -591,10 +664,14 @@ bool matmulTcEligible(const MatmulArgs& a) {
 bool matmulTcAligned(const MatmulArgs& a) { return rowsAligned(a.x, a.ldx) && rowsAligned(a.w, a.ldw); }
 
 cudaError_t launchMatmulTc(cudaStream_t st, const MatmulArgs& m) {
-  if(!matmulTcAligned(m)) return m.dt == DT_F16 ? launchWide<__half, true>(st, m) : launchWide<__nv_bfloat16, true>(st, m);
+  const bool plain = !matmulTcAligned(m);
   MatmulSkinnyArgs a = {};
   a.m = m;
-  if(skinnyShape(m, a)) return m.dt == DT_F16 ? launchSkinny<__half>(st, a) : launchSkinny<__nv_bfloat16>(st, a);
+  if(skinnyShape(m, plain, a)) {
+    if(plain) return m.dt == DT_F16 ? launchSkinny<__half, true>(st, a) : launchSkinny<__nv_bfloat16, true>(st, a);
+    return m.dt == DT_F16 ? launchSkinny<__half, false>(st, a) : launchSkinny<__nv_bfloat16, false>(st, a);
+  }
+  if(plain) return m.dt == DT_F16 ? launchWide<__half, true>(st, m) : launchWide<__nv_bfloat16, true>(st, m);
   return m.dt == DT_F16 ? launchWide<__half, false>(st, m) : launchWide<__nv_bfloat16, false>(st, m);
 }
 

@@ -80,6 +80,22 @@ def test_matmul_shared_sums(m, n, k):
     assert (wide[:, 0] == 7).all() and (wide[:, 1 + n:] == 7).all()
 
 
+# 16-bit rows on 4-byte boundaries and on none, in wide tiles and in shared sums; odd sums in rows of even length
+@pytest.mark.parametrize("dtype", ("fp16", "bf16"))
+@pytest.mark.parametrize("off", (0, 1, 2))
+@pytest.mark.parametrize("m,n,k", [(278, 308, 4706), (135, 102, 1442), (10, 16, 678), (16, 181, 236), (34, 204, 46), (541, 1213, 1268), (4001, 300, 391), (129, 70, 517), (128, 129, 130)])
+def test_matmul_rows_off_vectors(dtype, m, n, k, off):
+    g = seeded(dtype, m, n, k, off)
+    ld = (k + 1) // 2 * 2 + (2 if off < 2 else 3)
+    x, w = (torch.full((rows, ld), NAN, dtype=TYPES[dtype], device="cuda")[:, off:off + k] for rows in (m, n))
+    x.copy_(normal(g, m, k, dtype=dtype)), w.copy_(normal(g, n, k, dtype=dtype, scale=k ** -0.5))
+    bias, residual = normal(g, n), normal(g, m, n, dtype=dtype)
+    want, bound = matmul_reference(dtype, x, w, bias, 1, residual)
+    got = multiply(dtype, x, w, bias, 1, residual)
+    assert_within(got, want, bound)
+    assert torch.equal(multiply(dtype, x, w, bias, 1, residual), got), "the same sums every time"
+
+
 @pytest.mark.parametrize("dtype", ALL)
 def test_matmul_every_activation(dtype):
     g = seeded(dtype)
