@@ -7,6 +7,8 @@
 // registers.  All in fp32.  Keys behind a sequence's length and masked keys are not read: their rows of K and V are zeros
 // in shared memory, so that nothing in them (NaN, Inf) reaches a product.  fp32 rows of whole vectors are copied asynchronously, the next
 // tile's under this one's products (16 x 361 tokens and states, 6 heads of 64: 117 us, 133 us through registers).
+// Of the last tile only the sixteens of keys that it has are multiplied (60 x 413 tokens over 5 keys, 32 / 4 heads of 48 and 64: 297 us, 473 us with whole tiles; long sequences are the same
+// to 5 % slower; leaving them out of the copies and exponentials as well gives another 5 % there and costs long ones 10 %).
 //
 // A row's state is (maximum, sum, unnormalised output).  Where few rows have many keys the keys are cut into parts of `chunk`
 // keys, one block each; a part writes its state to the workspace and crossAttnJoinKernel adds the parts in order (crossAttnJoinManyKernel
@@ -133,8 +135,10 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
 #pragma unroll
     for(int c = 0; c < NC; c++) o[i][c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
+  const bool vecOut = ((uintptr_t)a.out & 15) == 0 && ((a.oB | a.oT | a.oH) & 3) == 0;  // rows of out, of whole vectors too
   const float scale = a.scale * 1.4426950408889634f;
   for(int kt = k0; kt < k1; kt += XS_KEYS) {
+    const int groups = min(4, (k1 - kt + 15) / 16);  // of 16 keys, that the tile has: what is behind them costs no products
     const uint8_t* on = sOk + (ASYNC ? ((kt - k0) / XS_KEYS & 1) * XS_KEYS : 0);
     uint8_t* onNext = sOk + (ASYNC ? XS_KEYS - (on - sOk) : 0);
     if(ASYNC) {
@@ -155,21 +159,27 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
     for(int i = 0; i < RI; i++)
 #pragma unroll
       for(int j = 0; j < 4; j++) s2[i][j] = make_float2(0.0f, 0.0f);
+    auto multiply = [&](auto count) {
+      constexpr int J = decltype(count)::value;
 #pragma unroll 4
-    for(int d = 0; d < pq - 4; d += 4) {
-      float4 qv[RI], kv[4];
+      for(int d = 0; d < pq - 4; d += 4) {
+        float4 qv[RI], kv[J];
 #pragma unroll
-      for(int i = 0; i < RI; i++) qv[i] = *reinterpret_cast<const float4*>(sQ + (ty * RI + i) * pq + d);
+        for(int i = 0; i < RI; i++) qv[i] = *reinterpret_cast<const float4*>(sQ + (ty * RI + i) * pq + d);
 #pragma unroll
-      for(int j = 0; j < 4; j++) kv[j] = *reinterpret_cast<const float4*>(sK + (tx + 16 * j) * pq + d);
+        for(int j = 0; j < J; j++) kv[j] = *reinterpret_cast<const float4*>(sK + (tx + 16 * j) * pq + d);
 #pragma unroll
-      for(int i = 0; i < RI; i++)
+        for(int i = 0; i < RI; i++)
 #pragma unroll
-        for(int j = 0; j < 4; j++) {
-          s2[i][j] = __ffma2_rn(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
-          s2[i][j] = __ffma2_rn(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
-        }
-    }
+          for(int j = 0; j < J; j++) {
+            s2[i][j] = __ffma2_rn(make_float2(qv[i].x, qv[i].y), make_float2(kv[j].x, kv[j].y), s2[i][j]);
+            s2[i][j] = __ffma2_rn(make_float2(qv[i].z, qv[i].w), make_float2(kv[j].z, kv[j].w), s2[i][j]);
+          }
+      }
+    };
+    if(groups > 2) multiply(std::integral_constant<int, 4>());
+    else if(groups == 2) multiply(std::integral_constant<int, 2>());
+    else multiply(std::integral_constant<int, 1>());
     float s[RI][4];
 #pragma unroll
     for(int i = 0; i < RI; i++)
@@ -209,7 +219,7 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
     if(ASYNC) xsWaitAllButOne();  // V
     __syncthreads();
     // Output channels: CG threads have four each (of every 64 where there are more); the other threads of a row share the keys.
-    for(int j = ks * 4; j < XS_KEYS; j += 4 * KS) {
+    for(int j = ks * 4; j < groups * 16; j += 4 * KS) {
       float4 p[RI];
 #pragma unroll
       for(int i = 0; i < RI; i++) p[i] = *reinterpret_cast<const float4*>(sP + (ty * RI + i) * PP + j);
@@ -271,6 +281,15 @@ __global__ void __launch_bounds__(XS_THREADS, RI == 1 ? (NC == 1 ? 4 : (NC == 2 
     T* out = (T*)a.out + blk.b * a.oB + (r / G) * a.oT + (blk.kvh * G + r % G) * a.oH;
     const bool live = total != 0.0f && (!a.queryMask || a.queryMask[(int64_t)blk.b * a.qLen + r / G] != 0.0f);
     const float inv = 1.0f / total;
+    if(ASYNC && vecOut) {
+#pragma unroll
+      for(int c = 0; c < NC; c++) {
+        const int d = c * 64 + cg * 4;
+        const float4 v = o[i][c];
+        if(d < a.dv && ks == 0) *reinterpret_cast<float4*>(out + d) = live ? make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      }
+      continue;
+    }
 #pragma unroll
     for(int c = 0; c < NC; c++)
 #pragma unroll

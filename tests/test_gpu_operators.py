@@ -401,6 +401,19 @@ def test_attention_layouts(dtype, layout, n, m, h, hk, d):
     assert_within(out, want, bound)
 
 
+# keys that end in each sixteenth of a tile, and rows of out on and off 16-byte boundaries behind inputs that are on them
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("layout", ("dense", "odd"))
+@pytest.mark.parametrize("n,m", [(70, 5), (3, 16), (70, 17), (90, 33), (5, 40), (70, 49), (33, 64), (70, 65), (20, 100), (90, 113)])
+def test_attention_short_keys(dtype, layout, n, m):
+    g, q, k, v = attention_inputs(dtype, 3, n, m, 4, 2, 48, 64, layout)
+    k_lengths = torch.tensor([m, max(m - 16, 1), 0], dtype=torch.int32, device="cuda")
+    k[1, max(m - 16, 1):], v[1, max(m - 16, 1):] = NAN, float("inf")
+    k[2], v[2] = NAN, NAN
+    want, bound = attention_reference(dtype, q, k, v, 0.2, k_lengths=k_lengths)
+    assert_within(attend(dtype, q, k, v, laid_out(empty_out(q, v), layout), 0.2, k_lengths=k_lengths), want, bound)
+
+
 @pytest.mark.parametrize("dtype", ALL)
 def test_attention_repeated_inputs(dtype):
     """Strides of 0: one set of keys for all sequences, one value row for all heads."""
