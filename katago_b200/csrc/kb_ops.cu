@@ -9,6 +9,7 @@
 #include <string>
 
 #include "../../include/kb_modelblob.h"
+#include "kb_box.h"
 #include "kb_engine.h"
 #include "kb_kernels.cuh"
 
@@ -47,18 +48,6 @@ void checkPointer(const char* op, const char* name, const void* p, size_t align)
   if(dev != cur) refuse(who() + " lies on device " + std::to_string(dev) + ", the current device is " + std::to_string(cur));
 }
 
-// A tensor [n[0]][n[1]][n[2]][width] with strides in elements; the last dimension is contiguous.
-struct Box {
-  const char* name;
-  const void* p;
-  int64_t n[3], s[3];
-  int64_t width;
-  size_t elem;
-  bool empty() const { return n[0] == 0 || n[1] == 0 || n[2] == 0 || width == 0; }
-  // bytes from the first element to behind the last one
-  int64_t bytes() const { return ((n[0] - 1) * s[0] + (n[1] - 1) * s[1] + (n[2] - 1) * s[2] + width) * (int64_t)elem; }
-};
-
 constexpr int64_t MAX_STRIDE = int64_t(1) << 40, MAX_BYTES = int64_t(1) << 46;
 
 void checkBox(const char* op, const Box& b, bool written) {
@@ -70,42 +59,9 @@ void checkBox(const char* op, const Box& b, bool written) {
   if(extent * (__int128)b.elem > MAX_BYTES) refuse(std::string(op) + ": " + b.name + " is too large");
   checkPointer(op, b.name, b.p, b.elem);
   if(!written) return;
-  // No two of its elements may be the same: from the smallest stride up, each clears what the dimensions below it span.
-  int order[3] = {0, 1, 2};
-  for(int i = 0; i < 3; i++)
-    for(int j = i + 1; j < 3; j++)
-      if(b.s[order[j]] < b.s[order[i]]) std::swap(order[i], order[j]);
-  int64_t span = b.width;
-  for(int i = 0; i < 3; i++) {
-    const int d = order[i];
-    if(b.n[d] <= 1) continue;
-    if(b.s[d] < span) refuse(std::string(op) + ": rows of " + b.name + " overlap one another");
-    span += (b.n[d] - 1) * b.s[d];
-  }
+  if(overlapsItself(b)) refuse(std::string(op) + ": rows of " + b.name + " overlap one another");
 }
 
-// Whether two tensors may share an element.  Exact enough for parts of one buffer: channel ranges of the same rows do not.
-bool mayOverlap(const Box& a, const Box& b) {
-  if(a.empty() || b.empty()) return false;
-  const int64_t pa = (int64_t)(uintptr_t)a.p, pb = (int64_t)(uintptr_t)b.p;
-  if(pa + a.bytes() <= pb || pb + b.bytes() <= pa) return false;
-  // rows of the same stride (tokens, or sequences of one token; batches of whole rows): compare the windows that each takes of a row
-  auto rowOf = [](const Box& x) { return (x.n[1] > 1 ? x.s[1] : (x.n[0] > 1 ? x.s[0] : 0)) * (int64_t)x.elem; };
-  const int64_t ra = rowOf(a), rb = rowOf(b), row = std::max(ra, rb);
-  if(row <= 0 || (ra != 0 && ra != row) || (rb != 0 && rb != row)) return true;
-  auto whole = [](const Box& x) { return x.n[0] == 1 || x.n[1] == 1 || x.s[0] % x.s[1] == 0; };
-  if(!whole(a) || !whole(b)) return true;
-  const int64_t wa = ((a.n[2] - 1) * a.s[2] + a.width) * (int64_t)a.elem, wb = ((b.n[2] - 1) * b.s[2] + b.width) * (int64_t)b.elem;
-  if(wa > row || wb > row) return true;
-  const int64_t delta = (((pb - pa) % row) + row) % row;
-  return delta < wa || delta + wb > row;
-}
-bool sameBox(const Box& a, const Box& b) {
-  if(a.p != b.p) return false;
-  for(int i = 0; i < 3; i++)
-    if(a.n[i] > 1 && a.s[i] != b.s[i]) return false;
-  return true;
-}
 void checkApart(const char* op, const Box& out, const Box& in) {
   if(mayOverlap(out, in)) refuse(std::string(op) + ": " + out.name + " overlaps " + in.name);
 }

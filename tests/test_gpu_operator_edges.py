@@ -1,0 +1,31 @@
+"""kb_matmul, kb_rope and kb_cross_attention where their arithmetic ends: infinities, NaN, weights and angles at the edge of a type; and
+calls that share memory or a graph in unusual ways.  (Bounds: operator_cases.py.)"""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from katago_b200 import capi  # noqa: E402
+from tests.operator_cases import PRECISION, stream, view  # noqa: E402
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+
+# ---- memory that a call's tensors share ----
+
+def test_inputs_that_repeat_beside_the_output_in_one_buffer():
+    """A query that all tokens of a sequence share, interleaved with the output: refused, since its rows are further apart than the
+    output's.  In a buffer of its own it is taken."""
+    fp32 = PRECISION["fp32"]
+    whole = torch.zeros(2, 1 + 8, 64, device="cuda")
+    at, step = whole.data_ptr(), 9 * 64
+    repeated, out = capi.View(at, step, 0, 64), capi.View(at + 4 * 64, step, 64, 64)
+    pos, freqs = torch.zeros(8, 1, dtype=torch.int32, device="cuda"), torch.zeros(32, 1, device="cuda")
+    with pytest.raises(capi.KBError, match="q out overlaps q in"):
+        capi.rope(fp32, 2, 8, 64, 64, pos.data_ptr(), 0, 1, freqs.data_ptr(), 1, 0, repeated, out, 1, stream=stream())
+    kv = torch.ones(2, 5, 1, 64, device="cuda")
+    with pytest.raises(capi.KBError, match="out overlaps q"):
+        capi.cross_attention(fp32, 2, 8, 5, 1, 1, 64, 64, 1.0, repeated, view(kv), view(kv), out, stream=stream())
+    own = torch.ones(2, 64, device="cuda")
+    capi.cross_attention(fp32, 2, 8, 5, 1, 1, 64, 64, 1.0, capi.View(own.data_ptr(), 64, 0, 64), view(kv), view(kv), out, stream=stream())
+    assert (whole[:, 0] == 0).all() and (whole[:, 1:] - 1).abs().max() < 1e-6
