@@ -70,10 +70,6 @@ void checkCount(const char* op, const char* name, int64_t v, int64_t least, int6
   if(v < least || v > most) refuse(std::string(op) + ": " + name + " is " + std::to_string(v) + ", not in " + std::to_string(least) + ".." + std::to_string(most));
 }
 
-void checkVector(const char* op, const char* name, const void* p, size_t elem) {
-  if(p) checkPointer(op, name, p, elem);
-}
-
 Box boxOf(const char* name, const kb_view* v, int64_t batch, int64_t tokens, int64_t heads, int64_t width, size_t elem) {
   return Box{name, v->data, {batch, tokens, heads}, {v->batchStride, v->tokenStride, v->headStride}, width, elem};
 }
@@ -261,10 +257,14 @@ void opCrossAttn(CrossAttnArgs a, const kb_view* q, const kb_view* k, const kb_v
   checkApart(op, bo, bq);
   checkApart(op, bo, bk);
   checkApart(op, bo, bv);
-  checkVector(op, "qLengths", a.qLengths, 4);
-  checkVector(op, "kLengths", a.kLengths, 4);
-  checkVector(op, "keyMask", a.kLen > 0 ? a.keyMask : nullptr, 4);
-  checkVector(op, "queryMask", a.queryMask, 4);
+  const int64_t queries = (int64_t)a.batch * a.qLen, keys = (int64_t)a.batch * a.kLen;
+  const Box vectors[4] = {{"the query lengths", a.qLengths, {1, 1, 1}, {0, 0, 0}, a.batch, 4}, {"the key lengths", a.kLengths, {1, 1, 1}, {0, 0, 0}, a.batch, 4},
+                          {"the key mask", a.keyMask, {1, 1, 1}, {0, 0, 0}, keys, 4}, {"the query mask", a.queryMask, {1, 1, 1}, {0, 0, 0}, queries, 4}};
+  for(const Box& x : vectors)
+    if(x.p) {
+      checkBox(op, x, false);
+      checkApart(op, bo, x);
+    }
   const size_t need = crossAttnWorkspace(a.dt, a.batch, a.qLen, a.kLen, a.heads, a.kvHeads, a.dq, a.dv);
   if(need > 0) {
     if(workspaceBytes < need) refuse("kb_cross_attention: the workspace has " + std::to_string(workspaceBytes) + " bytes, " + std::to_string(need) + " are needed");
@@ -274,6 +274,8 @@ void opCrossAttn(CrossAttnArgs a, const kb_view* q, const kb_view* k, const kb_v
     checkApart(op, ws, bk);
     checkApart(op, ws, bv);
     checkApart(op, ws, bo);
+    for(const Box& x : vectors)
+      if(x.p) checkApart(op, ws, x);
   }
   a.q = q->data; a.qB = q->batchStride; a.qT = q->tokenStride; a.qH = q->headStride;
   a.k = k->data; a.kB = k->batchStride; a.kT = k->tokenStride; a.kH = k->headStride;

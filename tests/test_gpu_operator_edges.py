@@ -29,3 +29,27 @@ def test_inputs_that_repeat_beside_the_output_in_one_buffer():
     own = torch.ones(2, 64, device="cuda")
     capi.cross_attention(fp32, 2, 8, 5, 1, 1, 64, 64, 1.0, capi.View(own.data_ptr(), 64, 0, 64), view(kv), view(kv), out, stream=stream())
     assert (whole[:, 0] == 0).all() and (whole[:, 1:] - 1).abs().max() < 1e-6
+
+
+def test_lengths_and_masks_that_an_output_or_the_workspace_would_overwrite_are_refused():
+    fp32, b, n, m = PRECISION["fp32"], 2, 3, 5000
+    q, k = torch.zeros(b, n, 1, 16, device="cuda"), torch.zeros(b, m, 1, 16, device="cuda")
+    room = capi.cross_attention_workspace(fp32, b, n, m, 1, 1, 16, 16)
+    assert room > 0
+    out, space = torch.zeros(8 + b * n * 16, device="cuda")[8:].view(b, n, 1, 16), torch.zeros(room // 4, device="cuda")
+    lengths, keys, rows = torch.full((b,), m, dtype=torch.int32, device="cuda"), torch.ones(b, m, device="cuda"), torch.ones(b, n, device="cuda")
+
+    def call(**given):
+        capi.cross_attention(fp32, b, n, m, 1, 1, 16, 16, 1.0, view(q), view(k), view(k), view(out), workspace=space.data_ptr(), workspace_bytes=room,
+                             stream=stream(), **given)
+
+    names = dict(q_lengths="the query lengths", k_lengths="the key lengths", key_mask="the key mask", query_mask="the query mask")
+    for what, name in names.items():
+        for into, who in ((out, "out"), (space, "the workspace")):
+            with pytest.raises(capi.KBError, match=f"{who} overlaps {name}"):
+                call(**{what: into.data_ptr() + 8})
+    # the last element alone, behind the start of the output
+    with pytest.raises(capi.KBError, match="out overlaps the key lengths"):
+        call(k_lengths=out.data_ptr() - 4)
+    call(k_lengths=lengths.data_ptr(), key_mask=keys.data_ptr(), query_mask=rows.data_ptr())
+    torch.cuda.synchronize()
