@@ -82,8 +82,9 @@ __device__ __forceinline__ void tmemLd64Now(uint32_t taddr, uint32_t (&r)[64]) {
     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]) : "r"(taddr) : "memory");
 }
 
-// 2^t of two numbers t = 142 u - 126 up to 16 (twice what a maximum may lag), u cut to [0, 1]: below t = -126 as for -126.  A NaN does not survive it: rows that have one get a reference of NaN, which the exponentials of the special-function
-// units carry on.
+// 2^t of two numbers t = 142 u - 126 up to 16 (twice what a maximum may lag), u cut to [0, 1]: below t = -126 as for -126.  A NaN does not
+// survive it, neither one that was a score nor infinity - infinity: rows with a score that is NaN or +infinity get a reference of NaN, which
+// the exponentials of the special-function units carry on, whichever key it was.
 __device__ __forceinline__ float fmaSat(float a, float b, float c) {
   float d;
   asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -377,7 +378,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
           float keep = 1.0f;
           if(grow) {
             keep = exp2f(ref - now);
-            ref = now;
+            ref = now == INFINITY ? __int_as_float(0x7fffffff) : now;
             sum *= keep;
           }
           if(i > 0) {

@@ -6,9 +6,12 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from katago_b200 import capi  # noqa: E402
-from tests.operator_cases import PRECISION, stream, view  # noqa: E402
+from tests.operator_cases import PRECISION, assert_within, attend, attention_reference, stream, view  # noqa: E402
+from tests.test_gpu_operators import ALL, attention_inputs, empty_out  # noqa: E402
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
+
+INF = float("inf")
 
 
 # ---- memory that a call's tensors share ----
@@ -53,3 +56,33 @@ def test_lengths_and_masks_that_an_output_or_the_workspace_would_overwrite_are_r
         call(k_lengths=out.data_ptr() - 4)
     call(k_lengths=lengths.data_ptr(), key_mask=keys.data_ptr(), query_mask=rows.data_ptr())
     torch.cuda.synchronize()
+
+
+# ---- attention ----
+
+# one kernel after the other: few rows, one row tile whose keys two warpgroups share, two row tiles a block, both head sizes; CUDA cores
+SHAPES = [(1, 2, 2, 64), (3, 4, 2, 128), (40, 2, 2, 64), (40, 4, 2, 128), (300, 6, 6, 64), (300, 6, 6, 128), (20, 2, 2, 136), (2, 2, 2, 20)]
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+@pytest.mark.parametrize("at", (0, 130))
+def test_attention_of_infinite_scores(dtype, n, h, hk, d, at):
+    """Sixteen sequences with an infinity at another key each.  A score of +infinity makes its rows NaN (infinity - infinity), whichever key
+    it is; one of -infinity leaves its key out.  The other heads are as ever."""
+    _, q, k, v = attention_inputs(dtype, 16, n, 200, h, hk, d, d, at)
+    q[..., 0] = q[..., 0].abs() + 0.25
+    want, bound = attention_reference(dtype, q, k, v, d ** -0.5)
+    for sign in (1, -1):
+        kk = k.clone()
+        for i in range(16):
+            kk[i, at + i, 0, 0] = sign * INF
+        out = attend(dtype, q, kk, v, empty_out(q, v), d ** -0.5)
+        first = h // hk
+        if sign > 0:
+            assert out[:, :, :first].isnan().all()
+        else:
+            mask = torch.ones(16, 200, device="cuda")
+            mask[torch.arange(16), at + torch.arange(16)] = 0
+            assert_within(out[:, :, :first], *(t[:, :, :first] for t in attention_reference(dtype, q, k, v, d ** -0.5, key_mask=mask)))
+        assert_within(out[:, :, first:], want[:, :, first:], bound[:, :, first:])
