@@ -453,7 +453,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         sState[t * 256 + 128 + row] = sum;
         softmaxWarpgroupsSync();
         const float r0 = sState[row], r1 = sState[256 + row];
-        ref = fmaxf(r0, r1);
+        ref = max3Nan(r0, r1, r1);  // a NaN is seen even if the other warpgroup had no key
         const float from = ref == -INFINITY ? 0.0f : ref;
         w0 = exp2f(r0 - from);
         w1 = exp2f(r1 - from);

@@ -7,7 +7,7 @@ torch = pytest.importorskip("torch")
 
 from katago_b200 import capi  # noqa: E402
 from tests.operator_cases import PRECISION, assert_within, attend, attention_reference, stream, view  # noqa: E402
-from tests.test_gpu_operators import ALL, attention_inputs, empty_out  # noqa: E402
+from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out  # noqa: E402
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
 
@@ -86,3 +86,20 @@ def test_attention_of_infinite_scores(dtype, n, h, hk, d, at):
             mask[torch.arange(16), at + torch.arange(16)] = 0
             assert_within(out[:, :, :first], *(t[:, :, :first] for t in attention_reference(dtype, q, k, v, d ** -0.5, key_mask=mask)))
         assert_within(out[:, :, first:], want[:, :, first:], bound[:, :, first:])
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+@pytest.mark.parametrize("m", (300, 4000))
+@pytest.mark.parametrize("bad", (NAN, INF))
+def test_attention_nan_is_seen_where_all_other_tiles_are_left_out(dtype, n, h, hk, d, m, bad):
+    """Keys of one tile only, one of them NaN (or a score of infinity): whoever has the other tiles has nothing to add."""
+    _, q, k, v = attention_inputs(dtype, 2, n, m, h, hk, d, d)
+    q[..., 0] = q[..., 0].abs() + 0.25
+    mask = torch.zeros(2, m, device="cuda")
+    mask[0, 3:100] = 1
+    mask[1, 140:250] = 1
+    k[0, 50, 0, 0] = k[1, 200, 0, 0] = bad
+    out = attend(dtype, q, k, v, empty_out(q, v), d ** -0.5, key_mask=mask)
+    assert out[:, :, :h // hk].isnan().all()
+    assert torch.isfinite(out[:, :, h // hk:]).all()
