@@ -11,9 +11,11 @@
 //   computed before its product; with 128 there is no room, they lie over the scores, and the next scores follow the product.
 //   A block with one row tile gives the warpgroups every other tile of keys instead, and adds the two states at the end.
 //
-// The row maximum is kept in units of log2; p = 2^(scale log2(e) s - ref), where ref follows the maximum only when that has grown by
-// more than 8 (p stays below 2^8, sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O
-// through registers and a wait for the product before.  The factor cancels in O / sum.
+// p = 2^(scale log2(e) (s - ref)), where ref follows the row's maximum of s only when that has grown by more than 8 in the exponent (p stays
+// below 2^8, sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O through registers and a wait
+// for the product before.  The factor cancels in O / sum.  One multiply-add makes an exponent, from scale log2(e) ref rounded once.
+// Where that is above 512 its rounding would show (at 10^9 it is a hundred steps of the exponent): such a warp goes on
+// with a loop that subtracts ref from the scores first.
 //
 // Keys that are not attended (masked, or behind the last one) may hold anything.  In shared memory their rows of V are cleared and
 // their rows of K are replaced by that of an attended key of the tile: so their scores are scores of the row that lie no higher
@@ -47,6 +49,7 @@ namespace {
 constexpr int XT_THREADS = 384, XT_KEYS = 128, XT_ERR = 311;
 constexpr int XT_HALF = 128 * 64 * 2;  // bytes of 128 rows x 64 channels
 constexpr float XT_GROW = 8.0f;
+constexpr float XT_FAR = 512.0f;
 enum { XT_ALL, XT_SOME, XT_NONE };
 constexpr int XT_SORT = 128;  // sequences that a block ranks
 
@@ -82,9 +85,9 @@ __device__ __forceinline__ void tmemLd64Now(uint32_t taddr, uint32_t (&r)[64]) {
     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]) : "r"(taddr) : "memory");
 }
 
-// 2^t of two numbers t = 142 u - 126 up to 16 (twice what a maximum may lag), u cut to [0, 1]: below t = -126 as for -126.  A NaN does not
-// survive it, neither one that was a score nor infinity - infinity: rows with a score that is NaN or +infinity get a reference of NaN, which
-// the exponentials of the special-function units carry on, whichever key it was.
+// 2^t of two numbers up to 16 (twice what a maximum may lag), below t = -112 as for -112: t = 128 u - 112 with u cut to [0, 1], which costs no more
+// than 2^-18 of t.  A NaN does not survive it, neither one that was a score nor infinity - infinity: rows with a score that is NaN or
+// +infinity get a reference of NaN, which the exponentials of the special-function units carry on, whichever key it was.
 __device__ __forceinline__ float fmaSat(float a, float b, float c) {
   float d;
   asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -94,9 +97,9 @@ template <typename T> __device__ __forceinline__ float2 ex2Poly(float2 u) {
   constexpr bool LONG = std::is_same<T, __half>::value;
   auto both = [](float c) { return make_float2(c, c); };
   // 1.5 * 2^23: the sum's low bits are the nearest whole number
-  const float2 r = __ffma2_rn(u, both(142.0f), both(12582912.0f - 126.0f));
-  const float2 n = __fadd2_rn(r, both(-(12582912.0f - 126.0f)));
-  const float2 f = __ffma2_rn(u, both(142.0f), make_float2(-n.x, -n.y));
+  const float2 r = __ffma2_rn(u, both(128.0f), both(12582912.0f - 112.0f));
+  const float2 n = __fadd2_rn(r, both(-(12582912.0f - 112.0f)));
+  const float2 f = __ffma2_rn(u, both(128.0f), make_float2(-n.x, -n.y));
   float2 p;
   if(LONG) {
     p = __ffma2_rn(f, both(0.009570102207362652f), both(0.05591785907745361f));
@@ -350,9 +353,32 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
       const uint32_t tS = tmem + t * 128u + lanes, tO = tmem + Sh::O_AT + t * D + lanes, tP = tmem + Sh::P_AT + t * Sh::P_STEP + lanes;
       const float c = x.scale * 1.4426950408889634f;
       const float2 c2 = make_float2(c, c);
-      const float cu = c * (1.0f / 142.0f);
-      float ref = -INFINITY, sum = 0.0f;
-      bool ok = true;
+      const float cu = c * 0.0078125f;
+      float ref = -INFINITY, base = 0.0f, sum = 0.0f;
+      bool far = false, ok = true;  // far: one of this warp's references is above XT_FAR
+      auto grown = [&](float now) { return row < a.tileRows && ((now - ref) * c > XT_GROW || now != now); };
+      auto rescale = [&](int i, float now, bool grow) {  // the rows of this warp whose maximum has grown: false if a wait ran out
+        float keep = 1.0f;
+        if(grow) {
+          keep = exp2f((ref - now) * c);
+          ref = now == INFINITY ? __int_as_float(0x7fffffff) : now;
+          sum *= keep;
+        }
+        if(i == 0) return true;
+        const bool there = wait(&bO[t], (uint32_t)(i - 1) & 1u);
+        if(__any_sync(0xffffffffu, !there)) return false;
+        tcFenceAfter();
+#pragma unroll
+        for(int d = 0; d < D; d += 16) {
+          uint32_t o[16];
+          tmemLd16(tO + d, o);
+          tmemLdWaitFor(o);
+#pragma unroll
+          for(int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+          tmemSt16(tO + d, o);
+        }
+        return true;
+      };
       for(int i = 0; i < steps; i++) {
         const int j = keyTile(t, i);
         ok = wait(&bVReady[j % ST], (uint32_t)(j / ST) & 1u) && wait(&bS[t], (uint32_t)i & 1u);
@@ -360,33 +386,48 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         tcFenceAfter();
         const int kind = sKind[j % ST];
         uint32_t s[2][64];
-        tmemLd64Now(tS, s[0]);
-        tmemLd64Now(tS + 64u, s[1]);
-        if(Sh::APART) {  // the next scores may come
-          tcFenceBefore();
-          __syncwarp();
-          if(lane == 0) mbarArrive(smemU32(&bRead[t]));
-        }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        if(!far) {
+          tmemLd64Now(tS, s[0]);
+          tmemLd64Now(tS + 64u, s[1]);
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for(int k = 0; k < 2; k++)
+          for(int k = 0; k < 2; k++)
 #pragma unroll
-          for(int e = 0; e < 64; e += 2) top[(e / 2) & 3] = max3Nan(top[(e / 2) & 3], __uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1]));
-        const float now = kind == XT_NONE ? -INFINITY : max3Nan(max3Nan(top[0], top[1], top[2]), top[3], top[3]) * c;
-        const bool grow = row < a.tileRows && (now > ref + XT_GROW || now != now);
-        if(__any_sync(0xffffffffu, grow)) {
-          float keep = 1.0f;
-          if(grow) {
-            keep = exp2f(ref - now);
-            ref = now == INFINITY ? __int_as_float(0x7fffffff) : now;
-            sum *= keep;
+            for(int e = 0; e < 64; e += 2) top[(e / 2) & 3] = max3Nan(top[(e / 2) & 3], __uint_as_float(s[k][e]), __uint_as_float(s[k][e + 1]));
+          const float now = kind == XT_NONE ? -INFINITY : max3Nan(max3Nan(top[0], top[1], top[2]), top[3], top[3]);
+          const bool grow = grown(now);
+          if(__any_sync(0xffffffffu, grow)) {
+            far = __any_sync(0xffffffffu, grow && fabsf(now * c) > XT_FAR);
+            if(!far) {
+              ok = rescale(i, now, grow);
+              if(!ok) break;
+              base = ref == -INFINITY ? 0.0f : -ref * c;
+            }
           }
+        }
+        if(far) {
+          // the same with the reference subtracted from each score, in little code: unrolled like the other it costs that one's time (head
+          // size 64, 31 %; a warp that has come here stays)
+          float now = -INFINITY;
+#pragma unroll 1
+          for(uint32_t d = 0; d < 128u && kind != XT_NONE; d += 16u) {
+            uint32_t o[16];
+            tmemLd16(tS + d, o);
+            tmemLdWaitFor(o);
+#pragma unroll
+            for(int e = 0; e < 16; e += 2) now = max3Nan(now, __uint_as_float(o[e]), __uint_as_float(o[e + 1]));
+          }
+          const bool grow = grown(now);
           if(i > 0) {
             ok = wait(&bO[t], (uint32_t)(i - 1) & 1u);
             if(__any_sync(0xffffffffu, !ok)) { ok = false; break; }
             tcFenceAfter();
-#pragma unroll
-            for(int d = 0; d < D; d += 16) {
+          }
+          if(__any_sync(0xffffffffu, grow)) {
+            const float keep = grow ? exp2f((ref - now) * c) : 1.0f;
+            if(grow) { ref = now == INFINITY ? __int_as_float(0x7fffffff) : now; sum *= keep; }
+#pragma unroll 1
+            for(uint32_t d = 0; d < (uint32_t)D && i > 0; d += 16u) {
               uint32_t o[16];
               tmemLd16(tO + d, o);
               tmemLdWaitFor(o);
@@ -395,10 +436,43 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
               tmemSt16(tO + d, o);
             }
           }
+          const float from = ref == -INFINITY ? 0.0f : ref;
+#pragma unroll 1
+          for(uint32_t k = 0; k < 4u; k++) {
+            uint32_t o[2][16], p[16];
+            tmemLd16(tS + 32u * k, o[0]);
+            tmemLd16(tS + 32u * k + 16u, o[1]);
+            tmemLdWaitFor(o[0]);
+            tmemLdWaitFor(o[1]);
+#pragma unroll
+            for(int e = 0; e < 16; e++) {
+              const float* count = sCount + (j % ST) * XT_KEYS + 32 * k + 2 * e;
+              const float w0 = kind == XT_NONE ? 0.0f : ex2Approx((__uint_as_float(o[e >> 3][2 * (e & 7)]) - from) * c);
+              const float w1 = kind == XT_NONE ? 0.0f : ex2Approx((__uint_as_float(o[e >> 3][2 * (e & 7) + 1]) - from) * c);
+              sum += kind == XT_SOME ? w0 * count[0] + w1 * count[1] : w0 + w1;
+              p[e] = opPack<T>(w0, w1);
+            }
+            tmemSt16(tP + 16u * k, p);
+            if(k & 1u) {
+              tmemStWait();
+              tcFenceBefore();
+              __syncwarp();
+              if(lane == 0) mbarArrive(smemU32(&bP[2 * t + (k >> 1)]));
+            }
+          }
+          if(Sh::APART) {
+            __syncwarp();
+            if(lane == 0) mbarArrive(smemU32(&bRead[t]));
+          }
+          continue;
         }
-        const float base = ref == -INFINITY ? 0.0f : -ref;
+        if(Sh::APART) {  // the next scores may come
+          tcFenceBefore();
+          __syncwarp();
+          if(lane == 0) mbarArrive(smemU32(&bRead[t]));
+        }
         const float2 base2 = make_float2(base, base);
-        const float baseU = fmaf(base, 1.0f / 142.0f, 126.0f / 142.0f);  // (t + 126) / 142 lies in [0, 1] as far as t <= 16
+        const float baseU = fmaf(base, 0.0078125f, 0.875f);  // (t + 112) / 128 lies in [0, 1] as far as t <= 16
         float2 part[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
         if(Sh::APART && i > 0) {  // the product before has read the probabilities that these replace
           ok = wait(&bO[t], (uint32_t)(i - 1) & 1u);
@@ -455,8 +529,8 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
         const float r0 = sState[row], r1 = sState[256 + row];
         ref = max3Nan(r0, r1, r1);  // a NaN is seen even if the other warpgroup had no key
         const float from = ref == -INFINITY ? 0.0f : ref;
-        w0 = exp2f(r0 - from);
-        w1 = exp2f(r1 - from);
+        w0 = exp2f((r0 - from) * c);
+        w1 = exp2f((r1 - from) * c);
         sum = w0 * sState[128 + row] + w1 * sState[384 + row];
         ok = ok && wait(&bO[0], (uint32_t)(steps0 - 1) & 1u) && wait(&bO[1], (uint32_t)(steps1 - 1) & 1u);
       }
@@ -474,7 +548,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
       const float inv = live ? 1.0f / sum : 0.0f;
       float* part = a.sp.parts > 1 && mine ? xaPart(x, a.sp, blk, r, a.G) : nullptr;
       T* out = (T*)x.out + blk.b * x.oB + token * x.oT + head * x.oH;
-      if(part && (t == 0 || !cut)) { part[0] = ref; part[1] = sum; }
+      if(part && (t == 0 || !cut)) { part[0] = ref * c; part[1] = sum; }
 #pragma unroll
       for(int dd = 0; dd < D; dd += 16) {
         if(cut && dd >= D / 2) break;

@@ -1,13 +1,14 @@
 """kb_matmul, kb_rope and kb_cross_attention where their arithmetic ends: infinities, NaN, weights and angles at the edge of a type; and
 calls that share memory or a graph in unusual ways.  (Bounds: operator_cases.py.)"""
+import math
 
 import pytest
 
 torch = pytest.importorskip("torch")
 
 from katago_b200 import capi  # noqa: E402
-from tests.operator_cases import PRECISION, assert_within, attend, attention_reference, stream, view  # noqa: E402
-from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out  # noqa: E402
+from tests.operator_cases import PRECISION, TYPES, assert_within, attend, attention_reference, stream, view  # noqa: E402
+from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out, seeded  # noqa: E402
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
 
@@ -103,3 +104,67 @@ def test_attention_nan_is_seen_where_all_other_tiles_are_left_out(dtype, n, h, h
     out = attend(dtype, q, k, v, empty_out(q, v), d ** -0.5, key_mask=mask)
     assert out[:, :, :h // hk].isnan().all()
     assert torch.isfinite(out[:, :, h // hk:]).all()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+@pytest.mark.parametrize("size", (30.0, 3e3, 1e5, 3e7, 1e9))
+def test_attention_of_equal_large_scores(dtype, n, h, hk, d, size):
+    """All keys of a sequence are the same, so all scores are, however large: a row is the mean of the values.  Equal scores have equal errors, so the
+    bound (operator_cases.py) is that of the probabilities without that of the scores; 7.5e-5 more for the short polynomial of bf16."""
+    m = 300
+    _, q, k, v = attention_inputs(dtype, 2, n, m, h, hk, d, d, size)
+    root = math.sqrt(size)
+    q[:] = q * 0.01
+    q[..., 0] = root * (1 + 0.01 * torch.arange(n, device="cuda")[:, None] / n)
+    k[:] = k[:, :1] * 0.01
+    k[0, ..., 0], k[1, ..., 0] = root, -root
+    want = v.double().mean(1, keepdim=True).expand(-1, n, -1, -1).repeat_interleave(h // hk, 2)
+    a = v.double().abs().mean(1, keepdim=True).expand(-1, n, -1, -1).repeat_interleave(h // hk, 2)
+    u = torch.finfo(TYPES[dtype]).eps / 2
+    bound = a * 2 * ((u if dtype != "fp32" else 0) + 2.0 ** -19 + (7.5e-5 if dtype == "bf16" else 0) + (m + 8) * 2.0 ** -23)
+    out = attend(dtype, q, k, v, empty_out(q, v), 1.0)
+    assert_within(out, want, bound + u * (want.abs() + bound) + (2.0 ** -25 if dtype == "fp16" else 0))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+@pytest.mark.parametrize("at", (0, 130))
+def test_attention_of_one_key_far_above_the_others(dtype, n, h, hk, d, at):
+    """Finite inputs whose scores reach 10^9: a row is the value of its largest key, whichever of sixteen that is, in rows of every size.  Bound: the
+    probability, which need not be a power of two, is rounded to 16 bits in the sum of the values but not in the total (u, and 2^-19 for the
+    exponential, as in operator_cases.py), and the result is rounded."""
+    _, q, k, v = attention_inputs(dtype, 16, n, 200, h, hk, d, d, at)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 40000.0 * 2.0 ** -(torch.arange(n, device="cuda") % 8)[:, None]
+    k[..., 0] = -30000.0 * torch.rand(16, 200, 1, generator=seeded(n, h, d, at), device="cuda")
+    for i in range(16):
+        k[i, at + i, :, 0] = 31000.0 + 100 * i
+    want = torch.stack([v[i, at + i] for i in range(16)]).double()[:, None].expand(-1, n, -1, -1).repeat_interleave(h // hk, 2)
+    out = attend(dtype, q, k, v, empty_out(q, v), 1.0)
+    u = torch.finfo(TYPES[dtype]).eps / 2
+    bound = 2 * ((u if dtype != "fp32" else 0) + 2.0 ** -19) * want.abs()
+    assert_within(out, want, bound + u * (want.abs() + bound) + (2.0 ** -25 if dtype == "fp16" else 0))
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+@pytest.mark.parametrize("m", (700, 4000))
+@pytest.mark.parametrize("rising", (True, False))
+def test_attention_scores_that_grow_into_the_thousands(dtype, n, h, hk, d, m, rising):
+    """Small scores in some tiles of keys, thousands in others, with keys left out by masks and lengths in both, NaN and infinities in them."""
+    g, q, k, v = attention_inputs(dtype, 2, n, m, h, hk, d, d, rising)
+    steps = torch.linspace(0.05, 3000, m, device="cuda") if rising else torch.linspace(3000, 0.05, m, device="cuda")
+    k[0] = (k[0].float() * steps[:, None, None]).to(k.dtype)
+    k[1] = (k[1].float() * torch.where(torch.arange(m, device="cuda") < m // 2, 0.1, 2000.0)[:, None, None]).to(k.dtype)
+    mask = (torch.rand(2, m, generator=g, device="cuda") < 0.7).float()
+    mask[0, 128:260] = 0
+    lengths = torch.tensor([m - 37, m], dtype=torch.int32, device="cuda")
+    want, bound = attention_reference(dtype, q, k, v, 0.25, k_lengths=lengths, key_mask=mask)
+    left_out = (torch.arange(m, device="cuda") >= lengths[:, None]) | (mask == 0)
+    k[left_out], v[left_out] = NAN, INF
+    out = attend(dtype, q, k, v, empty_out(q, v), 0.25, k_lengths=lengths, key_mask=mask)
+    assert_within(out, want, bound)
+    # whatever the scores' own rounding does to the weights, a row lies between its values
+    kept = torch.where(left_out[..., None, None], 0, v).double().abs().amax(1, keepdim=True).repeat_interleave(h // hk, 2)
+    assert (out.double().abs() <= kept * 1.01).all()
