@@ -110,6 +110,9 @@ __global__ void __launch_bounds__(XF_THREADS, XfShape<D>::BLOCKS) crossAttnFewKe
     for(int e = 0; e < 4; e++) o[n][e] = 0.0f;
   float mx[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
   const float scale = a.scale * 1.4426950408889634f;
+  // Weights are at most 1, of the type of the product's operands.  In fp16 they are 2^15 times larger, and so are the sums that they cancel in: those
+  // that are 2^-29 of the maximum's still have all their bits.  (bf16 has the range of fp32.)
+  constexpr float UP = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 
   for(int i = 0; i < mine; i++) {
     asm volatile("cp.async.wait_group %0;" ::"n"(Sh::STAGES - 2) : "memory");
@@ -173,7 +176,7 @@ __global__ void __launch_bounds__(XF_THREADS, XfShape<D>::BLOCKS) crossAttnFewKe
     for(int n = 0; n < 2; n++)
 #pragma unroll
       for(int e = 0; e < 4; e++) {
-        s[n][e] = ex2Approx(s[n][e] - ref[e >> 1]);
+        s[n][e] = ex2Approx(s[n][e] - ref[e >> 1] + UP);
         sum[e >> 1] += s[n][e];  // this lane's keys
       }
     const uint32_t p[4] = {opPack<T>(s[0][0], s[0][1]), opPack<T>(s[0][2], s[0][3]), opPack<T>(s[1][0], s[1][1]), opPack<T>(s[1][2], s[1][3])};

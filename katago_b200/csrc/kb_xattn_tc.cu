@@ -11,8 +11,8 @@
 //   computed before its product; with 128 there is no room, they lie over the scores, and the next scores follow the product.
 //   A block with one row tile gives the warpgroups every other tile of keys instead, and adds the two states at the end.
 //
-// p = 2^(scale log2(e) (s - ref)), where ref follows the row's maximum of s only when that has grown by more than 8 in the exponent (p stays
-// below 2^8, sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O through registers and a wait
+// p = 2^(scale log2(e) (s - ref)), where ref follows the row's maximum of s only when that has grown by more than 8 in the exponent (fp16: 4;
+// sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O through registers and a wait
 // for the product before.  The factor cancels in O / sum.  One multiply-add makes an exponent, from scale log2(e) ref rounded once.
 // Where that is above 512 its rounding would show (at 10^9 it is a hundred steps of the exponent): such a warp goes on
 // with a loop that subtracts ref from the scores first.
@@ -48,7 +48,10 @@ namespace {
 
 constexpr int XT_THREADS = 384, XT_KEYS = 128, XT_ERR = 311;
 constexpr int XT_HALF = 128 * 64 * 2;  // bytes of 128 rows x 64 channels
-constexpr float XT_GROW = 8.0f;
+// Weights are 2^XT_UP times larger where they are fp16, and so are the sums that they cancel in: the largest are 2^15, those that
+// are 2^-25 of the reference's still have all their bits.  (bf16 has the range of fp32.)
+template <typename T> constexpr float XT_UP = std::is_same<T, __half>::value ? 11.0f : 0.0f;
+template <typename T> constexpr float XT_GROW = std::is_same<T, __half>::value ? 4.0f : 8.0f;  // of the exponent, before the reference follows
 constexpr float XT_FAR = 512.0f;
 enum { XT_ALL, XT_SOME, XT_NONE };
 constexpr int XT_SORT = 128;  // sequences that a block ranks
@@ -85,7 +88,7 @@ __device__ __forceinline__ void tmemLd64Now(uint32_t taddr, uint32_t (&r)[64]) {
     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]) : "r"(taddr) : "memory");
 }
 
-// 2^t of two numbers up to 16 (twice what a maximum may lag), below t = -112 as for -112: t = 128 u - 112 with u cut to [0, 1], which costs no more
+// 2^t of two numbers up to 16 (above what a maximum may lag), below t = -112 as for -112: t = 128 u - 112 with u cut to [0, 1], which costs no more
 // than 2^-18 of t.  A NaN does not survive it, neither one that was a score nor infinity - infinity: rows with a score that is NaN or
 // +infinity get a reference of NaN, which the exponentials of the special-function units carry on, whichever key it was.
 __device__ __forceinline__ float fmaSat(float a, float b, float c) {
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
       const float cu = c * 0.0078125f;
       float ref = -INFINITY, base = 0.0f, sum = 0.0f;
       bool far = false, ok = true;  // far: one of this warp's references is above XT_FAR
-      auto grown = [&](float now) { return row < a.tileRows && ((now - ref) * c > XT_GROW || now != now); };
+      auto grown = [&](float now) { return row < a.tileRows && ((now - ref) * c > XT_GROW<T> || now != now); };
       auto rescale = [&](int i, float now, bool grow) {  // the rows of this warp whose maximum has grown: false if a wait ran out
         float keep = 1.0f;
         if(grow) {
@@ -401,7 +404,7 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
             if(!far) {
               ok = rescale(i, now, grow);
               if(!ok) break;
-              base = ref == -INFINITY ? 0.0f : -ref * c;
+              base = ref == -INFINITY ? 0.0f : XT_UP<T> - ref * c;
             }
           }
         }
@@ -447,8 +450,8 @@ __global__ void __launch_bounds__(XT_THREADS, 1) crossAttnTcKernel(
 #pragma unroll
             for(int e = 0; e < 16; e++) {
               const float* count = sCount + (j % ST) * XT_KEYS + 32 * k + 2 * e;
-              const float w0 = kind == XT_NONE ? 0.0f : ex2Approx((__uint_as_float(o[e >> 3][2 * (e & 7)]) - from) * c);
-              const float w1 = kind == XT_NONE ? 0.0f : ex2Approx((__uint_as_float(o[e >> 3][2 * (e & 7) + 1]) - from) * c);
+              const float w0 = kind == XT_NONE ? 0.0f : ex2Approx(fmaf(__uint_as_float(o[e >> 3][2 * (e & 7)]) - from, c, XT_UP<T>));
+              const float w1 = kind == XT_NONE ? 0.0f : ex2Approx(fmaf(__uint_as_float(o[e >> 3][2 * (e & 7) + 1]) - from, c, XT_UP<T>));
               sum += kind == XT_SOME ? w0 * count[0] + w1 * count[1] : w0 + w1;
               p[e] = opPack<T>(w0, w1);
             }

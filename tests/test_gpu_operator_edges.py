@@ -168,3 +168,22 @@ def test_attention_scores_that_grow_into_the_thousands(dtype, n, h, hk, d, m, ri
     # whatever the scores' own rounding does to the weights, a row lies between its values
     kept = torch.where(left_out[..., None, None], 0, v).double().abs().amax(1, keepdim=True).repeat_interleave(h // hk, 2)
     assert (out.double().abs() <= kept * 1.01).all()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+@pytest.mark.parametrize("gap", (12.0, 17.95, 23.5))
+@pytest.mark.parametrize("m,every,at", [(8192, 8192, 0), (8192, 8192, 8191), (2000, 16, 0), (2000, 16, 15)])
+def test_attention_small_weights_that_add_up(dtype, n, h, hk, d, gap, m, every, at):
+    """Keys that take most of the weight (one, or one of every sixteen) and have values of 0, and thousands whose weights are 2^-gap of
+    theirs: what a row is, is their sum, so each of them has to be as good as the bound says (a rounding of u of itself, however small
+    it is)."""
+    _, q, k, v = attention_inputs(dtype, 2, n, m, h, hk, d, d, gap, every)
+    q[:], k[:] = 0, 0
+    q[..., 0] = 1
+    k[..., 0] = -gap * math.log(2.0)
+    v[:] = (v.abs() + 4) * 1024
+    k[:, at::every] = 0
+    v[:, at::every] = 0
+    want, bound = attention_reference(dtype, q, k, v, 1.0)
+    assert_within(attend(dtype, q, k, v, empty_out(q, v), 1.0), want, bound)
