@@ -214,8 +214,9 @@ int kb_matmul(
 
 /* Rotary positions with any number of axes (time, row, column): pair p of a head is turned by
  *   angle[b][t][p] = sum over a of positions[b][t][a] * freqs[table][p][a]     (x0, x1) -> (x0 cos - x1 sin, x0 sin + x1 cos)
- *   positions [batch][tokens][axes] int32, sequences posBatchStride apart (0: all have the same); any value: the angle is reduced
- *             to a fraction of a turn exactly, so far positions are as good as near ones
+ *   positions [batch][tokens][axes] int32, sequences posBatchStride apart (0: all have the same).  Any value: what counts is the
+ *             angle's fraction of a turn, which is off by no more than an fp32 rounding of it (2^-26 of a turn, and 2^-33 per axis) at the
+ *             farthest position as at the nearest, for frequencies up to 2^40
  *   freqs     [freqHeads][rotDim/2][axes] fp32, radians per step; head h of H uses table h*freqHeads/H (freqHeads divides qHeads
  *             and kHeads).  A pair that turns with one axis has zeros for the others
  *   pairsInHalves 0: pair p is channels 2p, 2p+1 (as in the nets of this library); 1: channels p, p + rotDim/2

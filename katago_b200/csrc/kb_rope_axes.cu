@@ -8,10 +8,11 @@
 //
 // Angles of far positions.  position * freq in fp32 is off by 2^-24 of the ANGLE: half a turn at a position of a few million.
 // Only the angle's fraction of a turn matters, and that is arithmetic modulo one: a frequency is turned into turns per step as
-// a 64-bit fixed-point fraction (computed in fp64 with the rest of 1/2pi behind its leading word), the product with an integer
-// position wraps by itself, and the sum over the axes does too.  What is left is a signed fraction of a turn, of which the upper
-// 32 bits go to sincospif: 2^-32 of a turn, at any int32 position (the frequency's own fraction is good to 2^-64, times a
-// position of 2^31 at worst 2^-33).
+// a 64-bit fixed-point fraction, the product with an integer position wraps by itself, and the sum over the axes does too.  The fraction
+// comes from two words in fp64 (the product with 1/2pi and what its rounding left, with the rest of 1/2pi), each of which is converted
+// by itself: it is good to 2^-64 of a turn, times a position of 2^31 at worst 2^-33 per axis.  Of the sum the upper 32 bits
+// go to sincospif as a float: off by 2^-32 of a turn, and by the float's rounding, 2^-26 of a turn at the most.  (Frequencies up to 2^40
+// radians per step; 1/2pi is known to 2^-110, which shows in larger ones.)
 #include "kb_kernels.cuh"
 #include "kb_ops.h"
 #include "kb_ops_dev.cuh"
@@ -26,31 +27,39 @@ namespace {
 constexpr double INV_2PI_HI = 0.15915494309189535;
 constexpr double INV_2PI_LO = -9.839338337591243e-18;
 
+// x, of size 1/2 at most, in units of 2^-64 to half a unit: scaled by 2^63 (no overflow at +-1/2), doubled in the ring, and the rest added.
+__device__ __forceinline__ unsigned long long ringOf(double x) {
+  const double units = x * 9223372036854775808.0, whole = rint(units);
+  return 2ull * (unsigned long long)__double2ll_rn(whole) + (unsigned long long)__double2ll_rn(2.0 * (units - whole));
+}
 // Turns per step of one position as a fraction of 2^64.
 __device__ __forceinline__ unsigned long long turnFraction(float freq) {
   const double f = (double)freq;
   const double hi = f * INV_2PI_HI;
   const double lo = fma(f, INV_2PI_HI, -hi) + f * INV_2PI_LO;
-  const double frac = (hi - rint(hi)) + lo;  // [-0.5, 0.5] and a little
-  // scaled by 2^63 (no overflow at +-0.5) and doubled in the ring
-  return 2ull * (unsigned long long)__double2ll_rn(frac * 9223372036854775808.0);
+  return ringOf(hi - rint(hi)) + ringOf(lo - rint(lo));
 }
 
 // Turn fractions that a block keeps in shared memory; more of them (many tables of many axes) are computed where they are used.
 constexpr int ROPE_TABLE = 4096;
 
 // MODE 0: scalar pairs (any alignment), 1: V elements = V/2 adjacent pairs per access, 2: halves, V pairs per two accesses
-template <typename T, int MODE, int V, bool COPY>
+// TABLE: the block keeps the turn fractions (the conversion in the token loop costs registers: 2 x 20 280 tokens 159 us with both, 124 us)
+template <typename T, int MODE, int V, bool COPY, bool TABLE>
 __global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const RopeArgs a, int chunks, int copies, int headsPerItem, long long items) {
   extern __shared__ unsigned long long sTurn[];  // [freqHeads][pairs][axes], or nothing
   gridDepLaunch();
   gridDepWait();
-  const long long entries = (long long)a.freqHeads * (a.rot / 2) * a.axes;
-  const bool table = entries <= ROPE_TABLE;
-  if(table) {
-    // the conversion of a frequency takes some ten fp64 operations: once per block, not once per token
-    for(int i = threadIdx.x; i < entries; i += 256) sTurn[i] = isfinite(a.freqs[i]) ? turnFraction(a.freqs[i]) : 0;
-    __syncthreads();
+  bool wild = !TABLE;  // some frequency may be infinite or a NaN
+  if(TABLE) {
+    const int entries = a.freqHeads * (a.rot / 2) * a.axes;
+    // the conversion of a frequency takes some twenty fp64 operations: once per block, not once per token
+    for(int i = threadIdx.x; i < entries; i += 256) {
+      const bool finite = isfinite(a.freqs[i]);
+      sTurn[i] = finite ? turnFraction(a.freqs[i]) : 0;
+      wild = wild || !finite;
+    }
+    wild = __syncthreads_or(wild);
   }
   constexpr int P = MODE == 0 ? 1 : (MODE == 1 ? V / 2 : V);
   const int pairs = a.rot / 2;
@@ -77,22 +86,20 @@ __global__ void __launch_bounds__(256, MODE == 2 ? 2 : 4) ropeAxesKernel(const R
       have = th;
       const long long first = ((long long)th * pairs + c * P) * a.axes;
       unsigned long long turn[P];
-      bool finite[P];
 #pragma unroll
-      for(int p = 0; p < P; p++) { turn[p] = 0; finite[p] = true; }
+      for(int p = 0; p < P; p++) turn[p] = 0;
       for(int x = 0; x < a.axes; x++) {
         const unsigned long long at = (unsigned long long)(long long)pos[x];
 #pragma unroll
-        for(int p = 0; p < P; p++) {
-          const float f = a.freqs[first + p * a.axes + x];
-          finite[p] = finite[p] && isfinite(f);
-          turn[p] += at * (table ? sTurn[first + p * a.axes + x] : turnFraction(finite[p] ? f : 0.0f));
-        }
+        for(int p = 0; p < P; p++) turn[p] += at * (TABLE ? sTurn[first + p * a.axes + x] : turnFraction(a.freqs[first + p * a.axes + x]));
       }
 #pragma unroll
       for(int p = 0; p < P; p++) {
         // upper 32 bits as a signed fraction: units of half a turn for sincospif
-        const float halfTurns = finite[p] ? (float)(int)(turn[p] >> 32) * 4.656612873077393e-10f : __int_as_float(0x7fffffff);
+        float halfTurns = (float)(int)(turn[p] >> 32) * 4.656612873077393e-10f;
+        if(wild)
+          for(int x = 0; x < a.axes; x++)
+            if(!isfinite(a.freqs[first + p * a.axes + x])) halfTurns = __int_as_float(0x7fffffff);
         sincospif(halfTurns, &sn[p], &cs[p]);
       }
     };
@@ -181,7 +188,8 @@ template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a)
   const int headsPerItem = (heads + groups - 1) / groups;
   const long long items = perHead * ((heads + headsPerItem - 1) / headsPerItem);
   const long long entries = (long long)a.freqHeads * (a.rot / 2) * a.axes;
-  const size_t smem = entries <= ROPE_TABLE ? (size_t)entries * 8 : 0;
+  const bool table = entries <= ROPE_TABLE;
+  const size_t smem = table ? (size_t)entries * 8 : 0;
   // Few blocks walk over the items, so that each converts the frequencies once.  Of 2 to 64 blocks per SM six were best: 128 x 361
   // tokens of 12 heads of 64 (fp16, 142 MB) 29.8 us, 31.4 us with as many as are resident.  So were four resident blocks for
   // adjacent pairs with three heads in flight (33 us with three blocks) and two for halves, which need their registers (2 x 20 280 tokens of 32
@@ -190,9 +198,13 @@ template <typename T> cudaError_t ropeLaunch(cudaStream_t st, const RopeArgs& a)
   const dim3 grid((unsigned)blocks), block(256);
   auto run = [&](auto kernel) { return launchDependent(kernel, grid, block, smem, st, a, chunks, copies, headsPerItem, items); };
   // (without channels to copy, a kernel without that loop: it costs the other one registers, 128 x 361 tokens 30 -> 32 us)
-  if(!vec) return copies ? run(ropeAxesKernel<T, 0, 1, true>) : run(ropeAxesKernel<T, 0, 1, false>);
-  if(a.halves) return copies ? run(ropeAxesKernel<T, 2, V, true>) : run(ropeAxesKernel<T, 2, V, false>);
-  return copies ? run(ropeAxesKernel<T, 1, V, true>) : run(ropeAxesKernel<T, 1, V, false>);
+  auto choose = [&](auto withTable) {
+    constexpr bool TABLE = decltype(withTable)::value;
+    if(!vec) return copies ? run(ropeAxesKernel<T, 0, 1, true, TABLE>) : run(ropeAxesKernel<T, 0, 1, false, TABLE>);
+    if(a.halves) return copies ? run(ropeAxesKernel<T, 2, V, true, TABLE>) : run(ropeAxesKernel<T, 2, V, false, TABLE>);
+    return copies ? run(ropeAxesKernel<T, 1, V, true, TABLE>) : run(ropeAxesKernel<T, 1, V, false, TABLE>);
+  };
+  return table ? choose(std::true_type()) : choose(std::false_type());
 }
 
 }  // namespace

@@ -1,6 +1,7 @@
 """kb_matmul, kb_rope and kb_cross_attention where their arithmetic ends: infinities, NaN, weights and angles at the edge of a type; and
 calls that share memory or a graph in unusual ways.  (Bounds: operator_cases.py.)"""
 import math
+from fractions import Fraction
 
 import pytest
 
@@ -8,7 +9,7 @@ torch = pytest.importorskip("torch")
 
 from katago_b200 import capi  # noqa: E402
 from tests.operator_cases import PRECISION, TYPES, assert_within, attend, attention_reference, stream, view  # noqa: E402
-from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out, seeded  # noqa: E402
+from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out, normal, seeded, turn  # noqa: E402
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
 
@@ -57,6 +58,52 @@ def test_lengths_and_masks_that_an_output_or_the_workspace_would_overwrite_are_r
         call(k_lengths=out.data_ptr() - 4)
     call(k_lengths=lengths.data_ptr(), key_mask=keys.data_ptr(), query_mask=rows.data_ptr())
     torch.cuda.synchronize()
+
+
+# ---- rope ----
+
+PI = Fraction(31415926535897932384626433832795028841971693993751058209749445923078164062862089986280348253421170679, 10 ** 100)
+
+
+def assert_turned_exactly(q, got, positions, freqs):
+    """Every pair (adjacent channels, one head) of q against its angle in whole numbers.  Bound: the angle is off by 2^-26 of a turn (9.4e-8) for
+    its rounding to fp32 and 2^-32 for its lower bits, sine and cosine by two steps (1.2e-7), and there are three roundings of 2^-24
+    (1.8e-7): 2^-21 (4.8e-7) of |x0| + |x1|, and 2^-24 of the result."""
+    for t in range(q.shape[1]):
+        for p in range(freqs.shape[1]):
+            total = sum(Fraction(int(positions[0, t, a])) * Fraction(float(freqs[0, p, a])) for a in range(freqs.shape[2]))
+            rest = float(total - math.floor(total / (2 * PI)) * 2 * PI)
+            x0, x1 = (float(q[0, t, 0, 2 * p + i]) for i in (0, 1))
+            for i, exact in ((0, x0 * math.cos(rest) - x1 * math.sin(rest)), (1, x0 * math.sin(rest) + x1 * math.cos(rest))):
+                allowed = (abs(x0) + abs(x1)) * 2.0 ** -21 + 2.0 ** -24 * abs(exact)
+                off = abs(float(got[0, t, 0, 2 * p + i]) - exact)
+                assert off <= allowed, (int(positions[0, t, 0]), float(freqs[0, p, 0]), off, allowed)
+
+
+@pytest.mark.parametrize("axes", (1, 3, 16))
+def test_rope_at_the_farthest_positions(axes):
+    """int32 positions to the last, frequencies of a quarter to half a turn: the angle is off by a fraction of an fp32 step of a turn there too,
+    however many axes add up."""
+    g = seeded(axes)
+    n, pairs = 24, 64
+    q = torch.zeros(1, n, 1, 2 * pairs, device="cuda")
+    q[..., 0::4] = q[..., 3::4] = 1  # (1, 0) and (0, 1)
+    positions = torch.randint(2 ** 30, 2 ** 31 - 1, (1, n, axes), generator=g, device="cuda").to(torch.int32)
+    positions[0, ::2] *= -1
+    positions[0, 0], positions[0, 1] = 2 ** 31 - 1, -2 ** 31
+    freqs = 1.6 + 1.5 * torch.rand(1, pairs, axes, generator=g, device="cuda")
+    got, _ = turn("fp32", q, None, positions, freqs, 2 * pairs, False)
+    assert_turned_exactly(q.cpu(), got.cpu(), positions.cpu(), freqs.cpu())
+
+
+def test_rope_of_large_frequencies():
+    """Many turns a step: what the two words of 1 / 2 pi say of a fraction of a turn is used to the last bit."""
+    g = seeded("large")
+    freqs = torch.tensor([12345.678, 3e6, 1e9, 2.0 ** 40, 1e13, 4.5e15, 3e16, 1.1e17, 7e17], device="cuda").view(1, 9, 1)
+    q = normal(g, 1, 40, 1, 18)
+    positions = torch.arange(-20, 20, device="cuda", dtype=torch.int32).view(1, 40, 1).contiguous()
+    got, _ = turn("fp32", q, None, positions, freqs, 18, False)
+    assert_turned_exactly(q.cpu(), got.cpu(), positions.cpu(), freqs.cpu())
 
 
 # ---- attention ----
