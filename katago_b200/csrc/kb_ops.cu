@@ -77,22 +77,9 @@ void needView(const char* op, const char* name, const kb_view* v) {
   if(v == nullptr) refuse(std::string(op) + ": " + name + " is NULL");
 }
 
-// A word of page-locked host memory that a kernel whose wait ran out writes and the next call reads.  One for the process,
-// made at the first use; a stream capture that is under way on the thread does not mind.
+// The word for the kernels of this call, after a look at what an earlier one has left there.
 int* waitStatus() {
-  static std::once_flag once;
-  static int* word = nullptr;
-  std::call_once(once, []() {
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    void* p = nullptr;
-    if(cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
-      word = static_cast<int*>(p);
-      *word = 0;
-    }
-    cudaThreadExchangeStreamCaptureMode(&mode);
-  });
-  if(!word) throw CudaError("page-locked memory for the status of device-side waits could not be allocated");
+  int* word = operatorWaitWord();
   const int code = __atomic_exchange_n(word, 0, __ATOMIC_ACQ_REL);
   if(code != 0) throw CudaError("a device-side wait timed out in an earlier operator call (code " + std::to_string(code) + "): its results are not valid");
   return word;
@@ -106,6 +93,23 @@ void checkLaunch(const char* op, cudaError_t e) {
 }
 
 }  // namespace
+
+int* operatorWaitWord() {
+  static std::once_flag once;
+  static int* word = nullptr;
+  std::call_once(once, []() {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    void* p = nullptr;
+    if(cudaHostAlloc(&p, 64, cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+      word = static_cast<int*>(p);
+      *word = 0;
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+  });
+  if(!word) throw CudaError("page-locked memory for the status of device-side waits could not be allocated");
+  return word;
+}
 
 cudaError_t SharedMemoryOptIn::operator()(const void* fn, int bytes) {
   int dev = 0;
@@ -213,6 +217,7 @@ void opRope(RopeArgs a, const kb_view* qIn, const kb_view* qOut, const kb_view* 
     checkApart(op, out[i], pos);
     checkApart(op, out[i], freqs);
   }
+  waitStatus();  // its own kernels wait for nothing; what it reads may come from one that did
   checkLaunch(op, launchRopeAxes(static_cast<cudaStream_t>(stream), a));
 }
 

@@ -12,6 +12,9 @@
 
 namespace kb {
 
+// A word of page-locked host memory that a kernel whose wait ran out writes and the next call of an operator reads.  One for the
+// process, made at the first use; a stream capture that is under way on the thread does not mind.
+int* operatorWaitWord();
 // Lets `fn` use up to `bytes` of shared memory on the current device; asked of the driver once per device.
 struct SharedMemoryOptIn {
   std::atomic<uint64_t> done{0};

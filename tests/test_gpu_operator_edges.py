@@ -1,5 +1,6 @@
 """kb_matmul, kb_rope and kb_cross_attention where their arithmetic ends: infinities, NaN, weights and angles at the edge of a type; and
 calls that share memory or a graph in unusual ways.  (Bounds: operator_cases.py.)"""
+import ctypes
 import math
 from fractions import Fraction
 
@@ -9,7 +10,7 @@ torch = pytest.importorskip("torch")
 
 from katago_b200 import capi  # noqa: E402
 from tests.operator_cases import PRECISION, TYPES, assert_within, attend, attention_reference, stream, view  # noqa: E402
-from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out, normal, seeded, turn  # noqa: E402
+from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out, multiply, normal, seeded, turn  # noqa: E402
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
 
@@ -58,6 +59,33 @@ def test_lengths_and_masks_that_an_output_or_the_workspace_would_overwrite_are_r
         call(k_lengths=out.data_ptr() - 4)
     call(k_lengths=lengths.data_ptr(), key_mask=keys.data_ptr(), query_mask=rows.data_ptr())
     torch.cuda.synchronize()
+
+
+# ---- a wait that ran out ----
+
+@pytest.mark.parametrize("op", ("matmul", "rope", "attention"))
+def test_a_wait_that_ran_out_is_reported_by_the_next_call_of_any_operator(op):
+    """The word that a kernel would leave its code in, set by hand: the next call says so and launches nothing, the one after is as ever."""
+    word = getattr(capi.lib(), "_ZN2kb16operatorWaitWordEv")
+    word.restype, word.argtypes = ctypes.c_void_p, []
+    t = torch.ones(1, 4, 1, 8, device="cuda")
+    pos, freqs = torch.zeros(4, 1, dtype=torch.int32, device="cuda"), torch.zeros(4, 1, device="cuda")
+
+    def call():
+        out = torch.zeros_like(t)
+        if op == "matmul":
+            multiply("fp32", t[0, :, 0], t[0, :, 0], y=out[0, :, 0, :4])
+        elif op == "rope":
+            capi.rope(PRECISION["fp32"], 1, 4, 8, 8, pos.data_ptr(), 0, 1, freqs.data_ptr(), 1, 0, view(t), view(out), 1, stream=stream())
+        else:
+            attend("fp32", t, t, t, out, 1.0)
+        return out
+
+    torch.cuda.synchronize()
+    ctypes.c_int.from_address(word()).value = 301
+    with pytest.raises(capi.KBError, match=r"wait timed out in an earlier operator call \(code 301\)"):
+        call()
+    assert call().abs().sum() > 0
 
 
 # ---- rope ----
