@@ -300,19 +300,29 @@ __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
         switch(a.m.act) {
           case KB_ACT_RELU:
 #pragma unroll
-            for(int j = 0; j < 32; j++) r[j] = __float_as_uint(fastAct(__uint_as_float(r[j]), KB_ACT_RELU));
+            for(int j = 0; j < 32; j++) r[j] = __float_as_uint(opFastAct(__uint_as_float(r[j]), KB_ACT_RELU));
             break;
           case KB_ACT_MISH:
 #pragma unroll
-            for(int j = 0; j < 32; j++) r[j] = __float_as_uint(fastAct(__uint_as_float(r[j]), KB_ACT_MISH));
+            for(int j = 0; j < 32; j += 2) {
+              float2 v = make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+              v = opFastMish(v, v);
+              r[j] = __float_as_uint(v.x);
+              r[j + 1] = __float_as_uint(v.y);
+            }
             break;
           case KB_ACT_SILU:
 #pragma unroll
-            for(int j = 0; j < 32; j++) r[j] = __float_as_uint(fastAct(__uint_as_float(r[j]), KB_ACT_SILU));
+            for(int j = 0; j < 32; j++) r[j] = __float_as_uint(opFastAct(__uint_as_float(r[j]), KB_ACT_SILU));
             break;
           case KB_ACT_MISH_SCALE8:
 #pragma unroll
-            for(int j = 0; j < 32; j++) r[j] = __float_as_uint(fastAct(__uint_as_float(r[j]), KB_ACT_MISH_SCALE8));
+            for(int j = 0; j < 32; j += 2) {
+              float2 v = make_float2(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
+              v = opFastMish(v, make_float2(8.0f * v.x, 8.0f * v.y));
+              r[j] = __float_as_uint(v.x);
+              r[j + 1] = __float_as_uint(v.y);
+            }
             break;
           default: break;
         }
@@ -542,7 +552,7 @@ __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
     alignas(8) T out[4];
 #pragma unroll
     for(int e = 0; e < 4; e++) {
-      f[e] = fastAct(f[e] + bias[e], a.m.act);
+      f[e] = opFastAct(f[e] + bias[e], a.m.act);
       if(res) f[e] += OpType<T>::to(old[e]);
       out[e] = OpType<T>::from(f[e]);
     }

@@ -40,16 +40,37 @@ template <typename T, int V> struct OpVec {
   __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<word*>(p) = w; }
 };
 
-// Activations: library functions for fp32 results, the special-function forms of the convolutions' epilogues for 16-bit ones (their
-// error is far below the rounding of the result).  mish(x) = x tanh(log(1 + e^x)) = x (n^2 + 2n) / (n^2 + 2n + 2) with n = e^x:
+// Activations: library functions for fp32 results, special-function forms as in the convolutions' epilogues for 16-bit ones (their
+// error is far below the rounding of the result).  A NaN stays one, +infinity too: fmaxf(NaN, 0) is 0, and x - 2xr is NaN for x = inf and
+// r = 0 where x (1 - 2r) is not.  mish(x) = x tanh(log(1 + e^x)) = x (n^2 + 2n) / (n^2 + 2n + 2) with n = e^x:
 // nothing cancels, and one exponential and a division take the place of exp, log1p and tanh.
 __device__ __forceinline__ float opMish(float x, float arg) {
   const float n = expf(fminf(arg, 30.0f));  // the quotient is 1 from about 9 on
   const float m = n * (n + 2.0f);
   return x * (m / (m + 2.0f));
 }
+__device__ __forceinline__ float opRelu(float x) {
+  float y;
+  asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(y) : "f"(x));
+  return y;
+}
+// x (1 - 2r), r = 1 / (n^2 + 2n + 2): two values with the packed fp32 instructions.
+__device__ __forceinline__ float2 opFastMish(float2 x, float2 arg) {
+  auto both = [](float c) { return make_float2(c, c); };
+  const float2 e = __fmul2_rn(arg, both(1.4426950408889634f));
+  const float2 n = make_float2(ex2Approx(e.x), ex2Approx(e.y));
+  const float2 d = __ffma2_rn(n, __ffma2_rn(n, both(-0.5f), both(-1.0f)), both(-1.0f));
+  return __fmul2_rn(x, __fadd2_rn(make_float2(rcpApprox(d.x), rcpApprox(d.y)), both(1.0f)));
+}
+__device__ __forceinline__ float opFastAct(float v, int act) {
+  if(act == KB_ACT_RELU) return opRelu(v);
+  if(act == KB_ACT_MISH) return opFastMish(make_float2(v, v), make_float2(v, v)).x;
+  if(act == KB_ACT_MISH_SCALE8) return opFastMish(make_float2(v, v), make_float2(8.0f * v, 8.0f * v)).x;
+  return fastAct(v, act);
+}
 template <typename T> __device__ __forceinline__ float opAct(float v, int act) {
-  if(sizeof(T) != 4) return fastAct(v, act);
+  if(sizeof(T) != 4) return opFastAct(v, act);
+  if(act == KB_ACT_RELU) return opRelu(v);
   if(act == KB_ACT_MISH) return opMish(v, v);
   if(act == KB_ACT_MISH_SCALE8) return opMish(v, 8.0f * v);
   return applyActF(v, act);
@@ -60,7 +81,7 @@ template <int U> __device__ __forceinline__ void opActF32(float (&v)[U], int act
   switch(act) {
     case KB_ACT_RELU:
 #pragma unroll
-      for(int u = 0; u < U; u++) v[u] = applyActF(v[u], KB_ACT_RELU);
+      for(int u = 0; u < U; u++) v[u] = opRelu(v[u]);
       break;
     case KB_ACT_SILU:
 #pragma unroll

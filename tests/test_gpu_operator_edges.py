@@ -88,6 +88,24 @@ def test_a_wait_that_ran_out_is_reported_by_the_next_call_of_any_operator(op):
     assert call().abs().sum() > 0
 
 
+# ---- matmul ----
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("m,n,k", [(3, 136, 72), (3, 65, 33), (12, 136, 4096), (40, 136, 2048), (300, 264, 72), (300, 65, 33), (3000, 1200, 64)])
+def test_matmul_activations_of_infinities_and_nan(dtype, m, n, k):
+    """relu, mish and silu of +infinity are +infinity, of NaN NaN: in the row that has it and nowhere else."""
+    g = seeded(dtype, m, n, k)
+    x, w, bias = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5), normal(g, n)
+    w[:, 5] = w[:, 5].abs() + 0.25
+    x[1, 5], x[2, 7] = INF, NAN
+    others = [i for i in range(m) if i not in (1, 2)]
+    for act in (1, 2, 3, 12):
+        y = multiply(dtype, x, w, bias, act)
+        assert (y[1] == INF).all(), act
+        assert y[2].isnan().all(), act
+        assert torch.isfinite(y[others]).all(), act
+
+
 # ---- rope ----
 
 PI = Fraction(31415926535897932384626433832795028841971693993751058209749445923078164062862089986280348253421170679, 10 ** 100)
