@@ -280,3 +280,35 @@ def test_attention_small_weights_that_add_up(dtype, n, h, hk, d, gap, m, every, 
     v[:, at::every] = 0
     want, bound = attention_reference(dtype, q, k, v, 1.0)
     assert_within(attend(dtype, q, k, v, empty_out(q, v), 1.0), want, bound)
+
+
+# ---- nets on boards that only this attention takes ----
+
+@pytest.mark.parametrize("precision,tolerance,floor,step", [(capi.PRECISION_FP32, 2e-4, 1.0, None), (capi.PRECISION_FP16, 0.03, 3.0, 2.0 ** -11), (capi.PRECISION_BF16, 0.2, 3.0, 2.0 ** -8)])
+@pytest.mark.parametrize("ylen,xlen", [(22, 22), (19, 25), (37, 20)])
+def test_attention_blocks_of_nets_on_large_boards(ylen, xlen, precision, tolerance, floor, step, oracle):
+    """Attention blocks of all kinds, boards of several sizes in one buffer, in every type against the oracle: element by element within the
+    reference's tolerance of a layer (cpp/tests/testnn.cpp:8-15, as for the other blocks), and on the whole within two steps of a 16-bit
+    type.  (Eight roundings of a value, of weights, inputs, queries, keys, values, probabilities and results, each off by half a step at
+    most and evenly spread, are sqrt(8 / 12) = 0.8 steps.)"""
+    import numpy as np
+
+    from katago_b200 import modelfile as mf
+    from tests.test_gpu_parity import _attn_block
+    g, rng = mf._Gen(78), np.random.default_rng(ylen * xlen)
+    mask = np.zeros((3, ylen, xlen), np.float32)
+    mask[0] = 1
+    mask[1, :13, :xlen - 2] = 1
+    mask[2, :ylen - 7, :9] = 1
+    on = mask > 0.5
+    for channels, layer in [(384, _attn_block(g, 384, 6, 6, 64, 64, "learnable")), (384, _attn_block(g, 384, 6, 2, 64, 64, "fixed")),
+                            (96, _attn_block(g, 96, 6, 3, 32, 16, "fixed")), (256, _attn_block(g, 256, 2, 2, 128, 128, "none"))]:
+        x = rng.standard_normal((3, ylen, xlen, channels)).astype(np.float32) * mask[..., None]
+        blob = mf.layer_blob(layer)
+        ref = oracle.eval_layer(blob, x, mask, channels)
+        out = capi.eval_layer(blob, x, mask, channels, precision=precision)
+        assert np.isfinite(out).all() and (out[~on] == 0).all()
+        assert np.all(np.abs(out - ref) <= tolerance * np.maximum(np.maximum(np.abs(out), np.abs(ref)), floor)), (channels, np.abs(out - ref).max())
+        if step:
+            off = np.sqrt(np.mean((out - ref)[on] ** 2) / np.mean(ref[on] ** 2))
+            assert off <= 2 * step, (channels, off / step)
