@@ -230,7 +230,7 @@ int kb_rope(
 /* Attention of qLen tokens to the kLen states of another sequence (or of their own):
  *   out[b][i][h] = sum over j of p[j] v[b][j][g],  p = softmax over j of scale * q[b][i][h] . k[b][j][g],  g = h*kvHeads/heads
  *   q [batch][qLen][heads][qkDim]   k [batch][kLen][kvHeads][qkDim]   v [batch][kLen][kvHeads][vDim]
- *   out [batch][qLen][heads][vDim]  head sizes 1..256, heads a multiple of kvHeads, scale > 0
+ *   out [batch][qLen][heads][vDim]  head sizes 1..256, heads a multiple of kvHeads, scale > 0 and at most 2.35e38
  *   qLengths, kLengths [batch] int32 on the device or NULL: rows of `out` from qLengths[b] on are left as they are; keys from
  *             kLengths[b] on are left out, whatever they hold.  Values outside 0..qLen / 0..kLen count as the nearer end
  *   keyMask   [batch][kLen] fp32 or NULL: keys whose mask is 0 are left out, whatever their k and v hold (NaN and Inf included)

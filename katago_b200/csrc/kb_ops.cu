@@ -247,7 +247,8 @@ void opCrossAttn(CrossAttnArgs a, const kb_view* q, const kb_view* k, const kb_v
   const char* op = "kb_cross_attention";
   const size_t es = elementSize(a.dt, op);
   checkAttnSizes(op, a.batch, a.qLen, a.kLen, a.heads, a.kvHeads, a.dq, a.dv);
-  if(!(a.scale > 0.0f) || a.scale > 3.0e38f) refuse("kb_cross_attention: the scale is not a positive number");
+  // (exponents are scores times scale log2(e), which has to be a number)
+  if(!(a.scale > 0.0f) || a.scale > 2.35e38f) refuse("kb_cross_attention: the scale is not a positive number up to 2.35e38");
   if(a.batch == 0 || a.qLen == 0) return;
   needView(op, "q", q);
   needView(op, "k", k);
