@@ -281,6 +281,112 @@ def test_attention_small_weights_that_add_up(dtype, n, h, hk, d, gap, m, every, 
     want, bound = attention_reference(dtype, q, k, v, 1.0)
     assert_within(attend(dtype, q, k, v, empty_out(q, v), 1.0), want, bound)
 
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+def test_attention_of_tokens_that_hold_nothing_and_rows_of_minus_infinity(dtype, n, h, hk, d):
+    """What a masked token and one behind the last hold (NaN, infinities) reaches no other row; a row all of whose scores are -infinity has no
+    key left, and is zeros."""
+    _, q, k, v = attention_inputs(dtype, 3, n, 300, h, hk, d, d)
+    tokens = torch.tensor([n, max(1, n // 2), n], dtype=torch.int32, device="cuda")
+    live = (torch.arange(n, device="cuda") % 3 != 1).float().expand(3, n).contiguous()
+    want, bound = attention_reference(dtype, q, k, v, 0.125, query_mask=live)
+    nothing = torch.tensor([NAN, INF, -INF, 60000.0], device="cuda")[torch.arange(n, device="cuda") % 4].to(q.dtype)[None, :, None, None]
+    dead = (live == 0) | (torch.arange(n, device="cuda") >= tokens[:, None])
+    q = torch.where(dead[..., None, None], nothing, q)
+    out = torch.full_like(empty_out(q, v), 7.0)
+    attend(dtype, q, k, v, out, 0.125, q_lengths=tokens, query_mask=live)
+    for i in range(3):
+        rows = int(tokens[i])
+        assert_within(out[i, :rows].flatten(0, 1), want[i, :rows].flatten(0, 1), bound[i, :rows].flatten(0, 1))
+        assert (out[i, rows:] == 7.0).all()
+    q[:], k[0] = 1, -INF
+    out = attend(dtype, q, k, v, empty_out(q, v), 0.125)
+    assert (out[0] == 0).all() and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("n,h,hk,d", SHAPES)
+@pytest.mark.parametrize("scale", (1e-45, 1e-30, 1e30))
+def test_attention_of_tiny_and_huge_scales(dtype, n, h, hk, d, scale):
+    """A scale of next to nothing makes a row the mean of its values; a huge one brings back scores that are next to nothing."""
+    m = 300
+    _, q, k, v = attention_inputs(dtype, 2, n, m, h, hk, d, d, scale)
+    if scale < 1:
+        want, bound = attention_reference(dtype, q * 0, k, v, 1.0)
+    elif dtype == "fp16":
+        return  # its products are never that small
+    else:
+        q, k = q * 1e-15, k * 1e-15
+        want, bound = attention_reference(dtype, q, k, v, scale)
+    assert_within(attend(dtype, q, k, v, empty_out(q, v), scale), want, bound)
+
+
+# ---- graphs ----
+
+def test_a_capture_that_forks_and_joins():
+    """Operators on two streams of one capture, behind and before each other and torch's own kernels, each with a workspace of its own."""
+    g = seeded("fork")
+    x, w = normal(g, 200, 512, dtype="fp16"), normal(g, 256, 512, dtype="fp16", scale=0.04)
+    q, kv = normal(g, 2, 3, 4, 64, dtype="fp16"), normal(g, 2, 6000, 4, 64, dtype="fp16")
+    side = torch.cuda.Stream()
+
+    def work(forked):
+        here = torch.cuda.current_stream()
+        a = multiply("fp16", x, w)
+        there = side if forked else here
+        there.wait_stream(here)
+        with torch.cuda.stream(there):
+            b = attend("fp16", q, kv, kv, empty_out(q, kv), 0.125)
+            c = a * 2
+            d = multiply("fp16", c, w[:, :256], act=3)
+        e = attend("fp16", q, kv, kv, empty_out(q, kv), 0.25)
+        here.wait_stream(there)
+        return a, b, c, d, e, multiply("fp16", d, w[:, 256:], residual=a)
+
+    want = [t.clone() for t in work(False)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(True)
+    for _ in range(20):
+        for t in got:
+            t.fill_(NAN)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
+FIRST_CALL = """
+import torch
+from tests.operator_cases import *
+from tests.test_gpu_operators import *
+g = seeded(1)
+x, w = normal(g, 200, 512, dtype="fp16"), normal(g, 256, 512, dtype="fp16")
+f, q, kv = x[:5].float(), normal(g, 2, 40, 4, 64, dtype="bf16"), normal(g, 2, 300, 4, 64, dtype="bf16")
+positions, freqs = angles_for(g, 2, 40, 2, 1, 32, 100)
+def work():
+    return multiply("fp16", x, w), multiply("fp32", f, f), attend("bf16", q, kv, kv, empty_out(q, kv), 0.125), turn("bf16", q, None, positions, freqs, 64, False)[0]
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    got = work()
+for t in got: t.zero_()
+graph.replay()
+for a, b in zip(got, work()):
+    assert torch.equal(a, b) and a.abs().sum() > 0
+print("captured")
+"""
+
+
+def test_the_first_call_of_a_process_may_be_captured():
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
 
 # ---- nets on boards that only this attention takes ----
 
