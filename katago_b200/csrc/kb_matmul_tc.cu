@@ -5,7 +5,8 @@
 // accumulators in tensor memory, sixteen warps take the other accumulator out: 32 rows x 32 columns at a time, each warp on its
 // own, through a slot of its own that TMA empties.  The residual arrives by TMA too, a unit ahead in another slot where a tile's
 // products are short, in the same slot where they are long.  Where y's rows are not on 16-byte boundaries the warp reads the
-// residual and writes the slot's rows itself, a row per instruction.  (Eight warps, 32 or 64 columns at a time: 46208 x 1024 x 384
+// residual and writes the slot's rows itself, a row per instruction; so it writes the last unit of rows that end inside sixteen bytes, since a
+// TMA store writes those sixteen whole, whatever lies behind the row's end.  (Eight warps, 32 or 64 columns at a time: 46208 x 1024 x 384
 // fp16 66 us with bias and SiLU; a warp's own chain of waits and special functions was what took the time.)
 //
 // Rows on other boundaries (PLAIN, both kernels): eight warps take the place of TMA and write the swizzled 128 bytes of a row that it would
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
           w.w = opPack<T>(__uint_as_float(r[8 * q + 6]), __uint_as_float(r[8 * q + 7]));
           *reinterpret_cast<uint4*>(mine + ((q ^ sw) << 4)) = w;
         }
-        if(a.tmaOut) {
+        if(a.tmaOut && (nc + MT_UNIT <= a.m.N || (a.m.N & 7) == 0)) {
           fenceProxyAsync();
           __syncwarp();
           if(electOne()) {

@@ -9,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 from katago_b200 import capi  # noqa: E402
-from tests.operator_cases import PRECISION, TYPES, assert_within, attend, attention_reference, stream, view  # noqa: E402
+from tests.operator_cases import PRECISION, TYPES, assert_within, attend, attention_reference, matmul_reference, stream, view  # noqa: E402
 from tests.test_gpu_operators import ALL, NAN, attention_inputs, empty_out, multiply, normal, seeded, turn  # noqa: E402
 
 pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs a CUDA device")]
@@ -104,6 +104,27 @@ def test_matmul_activations_of_infinities_and_nan(dtype, m, n, k):
         assert (y[1] == INF).all(), act
         assert y[2].isnan().all(), act
         assert torch.isfinite(y[others]).all(), act
+
+@pytest.mark.parametrize("dtype", ALL)
+@pytest.mark.parametrize("m,k", [(1, 72), (3, 72), (20, 72), (20, 2048), (129, 40), (300, 72), (300, 2048), (700, 33), (3000, 136), (140, 2048)])
+@pytest.mark.parametrize("n", (1, 3, 6, 33, 62, 100, 257, 1203))
+def test_matmul_writes_its_columns_only(dtype, m, k, n):
+    """Rows of y on 16-byte boundaries, an end of no whole vector: what lies behind it in the same sixteen bytes belongs to somebody else."""
+    g = seeded(dtype, m, n, k)
+    x, w = normal(g, m, k, dtype=dtype), normal(g, n, k, dtype=dtype, scale=k ** -0.5)
+    other = normal(g, m, n, dtype=dtype)
+    ld = (n + 7) // 8 * 8 + 8
+    for residual in ("none", "other", "itself"):
+        whole = torch.full((m, ld), 7.0, dtype=TYPES[dtype], device="cuda")
+        y = whole[:, :n]
+        if residual == "itself":
+            y.copy_(other)
+        padded = torch.full((m, ld), NAN, dtype=TYPES[dtype], device="cuda")
+        padded[:, :n] = other
+        r = dict(none=None, other=padded[:, :n], itself=y)[residual]
+        want, bound = matmul_reference(dtype, x, w, None, 0, None if r is None else r.clone())
+        assert_within(multiply(dtype, x, w, None, 0, r, y), want, bound, residual)
+        assert (whole[:, n:] == 7.0).all(), residual
 
 
 # ---- rope ----
