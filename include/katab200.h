@@ -184,8 +184,10 @@ const char* kb_conv_noalloc_last_error(void);
  * Conventions of all of them:
  *   - pointers are DEVICE addresses on the current device (managed memory is taken too); host memory and memory of another
  *     device are refused.  Elements have the type that `precision` (KB_PRECISION_*) names, sums are held in fp32, a result is
- *     rounded once;
- *   - strides count elements and may be anything from 0 up for inputs (0 repeats); the innermost dimension is contiguous;
+ *     rounded once (attention of 16-bit types also rounds a key's weight to 16 bits before it meets the value; the total of the
+ *     weights takes them unrounded);
+ *   - strides count elements and may be anything from 0 up for inputs (0 repeats; the row strides of kb_matmul are at least a
+ *     row's length); the innermost dimension is contiguous;
  *     elements of an output must not coincide, and an output must not overlap an input or another output unless the text below
  *     allows it.  Column ranges of one buffer do not overlap if the tensors have the same row stride; tensors interleaved in some
  *     other way are refused, since that cannot be told from an overlap;
@@ -235,7 +237,7 @@ int kb_rope(
  *             kLengths[b] on are left out, whatever they hold.  Values outside 0..qLen / 0..kLen count as the nearer end
  *   keyMask   [batch][kLen] fp32 or NULL: keys whose mask is 0 are left out, whatever their k and v hold (NaN and Inf included)
  *   queryMask [batch][qLen] fp32 or NULL: tokens whose mask is 0 get a row of zeros
- * A row that no key is left for is zeros.
+ * A row that no key is left for is zeros, and so is one all of whose scores are -infinity; one with a score that is NaN or +infinity is NaN.
  *   workspace, workspaceBytes: device memory, 16-byte aligned, at least what kb_cross_attention_workspace says for the same sizes
  *             (it depends on nothing else; 0 for most).  Its contents need not be set and mean nothing after the call; two
  *             calls whose kernels overlap on the GPU (two streams, two graphs) need one each. */

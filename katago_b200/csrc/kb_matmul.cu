@@ -14,7 +14,7 @@
 //                    per lane: the sum over K may be taken in any order, so the lane that has channels 8t..8t+7 of a weight row
 //                    feeds them as four pairs wherever the instruction wants pairs, and the lane of a row of x does the same.
 //                    4 x 1024 x 384 bf16: 2.1 us, 4.0 us in kb_matmul_tc.cu; the two meet at 4 x 16384 x 512 (4.9 us), and longer
-//                    sums are better off with asynchronous copies (4 x 4096 x 4096: 12.8 us here, 9.2 us there).
+//                    sums are better off with asynchronous copies (4 x 4096 x 4096: 12.8 us here, 8.2 us there).
 #include "kb_kernels.cuh"
 #include "kb_ops.h"
 #include "kb_ops_dev.cuh"

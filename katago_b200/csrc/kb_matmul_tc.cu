@@ -7,7 +7,8 @@
 // products are short, in the same slot where they are long.  Where y's rows are not on 16-byte boundaries the warp reads the
 // residual and writes the slot's rows itself, a row per instruction; so it writes the last unit of rows that end inside sixteen bytes, since a
 // TMA store writes those sixteen whole, whatever lies behind the row's end.  (Eight warps, 32 or 64 columns at a time: 46208 x 1024 x 384
-// fp16 66 us with bias and SiLU; a warp's own chain of waits and special functions was what took the time.)
+// fp16 66 us with bias and SiLU, 51 us with sixteen, in the first milliseconds; 60 us over seconds, at the power limit.  A warp's own chain of
+// waits and special functions was what took the time.)
 //
 // Rows on other boundaries (PLAIN, both kernels): eight warps take the place of TMA and write the swizzled 128 bytes of a row that it would
 // have.  Rows on 4-byte boundaries go by asynchronous copies of two channels per lane (4096 x 4096 x 4098 bf16 860 us, 160 TFLOP/s;

@@ -29,7 +29,7 @@
 // cycles with head size 64 and 3200 with 128; the special-function units (16 exponentials per clock and SM, 2048 cycles) are the
 // busiest part.  So one pair of exponentials in eight is computed on the FMA units (t = n + f with n whole and |f| <= 1/2, 2^f by a
 // polynomial, n added to the exponent's bits): 2 x 4096 x 8192 tokens, 16 heads of 128, bf16: 520 us with none, 493 with one, 511 with
-// two, 540 with three.  The polynomials are minimax fits of the relative error over [-1/2, 1/2] (Remez exchange): degree 3 is off by
+// two, 540 with three (in the first milliseconds; 514 us with one over seconds, at the power limit).  The polynomials are minimax fits of the relative error over [-1/2, 1/2] (Remez exchange): degree 3 is off by
 // 7.5e-5 at most, for bf16 probabilities, whose rounding is 3.9e-3; degree 4 by 2.6e-6, for fp16 with 4.9e-4.
 // What did not help: four threads' warps to a scheduler (a row by two threads, 70 us where this takes 57); an issuing warp per row tile.
 //
