@@ -268,7 +268,8 @@ __global__ void __launch_bounds__(MT_THREADS, 1) matmulTcKernel(
         if(electOne()) requestResidual(group);
         asked++;
       }
-      ok = wait(&bAcc[b], (n >> 1) & 1u);
+      // (by TMA the longest sums that memory has room for take some 0.3 s, and the longer wait costs the others 2 %)
+      ok = PLAIN ? opWaitSums(smemU32(&bAcc[b]), (n >> 1) & 1u, abortFlag, a.m.status, MT_ERR, a.kSlices) : wait(&bAcc[b], (n >> 1) & 1u);
       if(__any_sync(0xffffffffu, !ok)) ok = false;
       tcFenceAfter();
       for(int c = group; c < nUnits && ok; c += MT_GROUPS, u++) {
@@ -503,7 +504,7 @@ __global__ void __launch_bounds__(MS_THREADS, 2) matmulSkinnyKernel(
   bool ok = true;
   if(warp >= 2) {
     const int quarter = warp & 3, half = (warp - 2) >> 2;
-    ok = wait(&bAcc, 0);
+    ok = opWaitSums(smemU32(&bAcc), 0, abortFlag, a.m.status, MS_ERR, s1 - s0);
     if(__any_sync(0xffffffffu, !ok)) ok = false;
     tcFenceAfter();
     for(int c = half * 16; c < rows && ok; c += 32) {

@@ -111,11 +111,11 @@ __device__ __forceinline__ float ldCluster1(uint32_t addr) {
   return v;
 }
 
-// Bounded wait of a role of these kernels (about 2 s).  A wait that runs out raises the abort flag and leaves `code` in the status
+// Bounded wait of a role of these kernels (about 2 s, or limitNs).  A wait that runs out raises the abort flag and leaves `code` in the status
 // word, which is page-locked host memory (hence a plain store); it returns false, as does one that finds the flag raised, and
 // the role then leaves its loops.
 // The clock is read only after some dozens of tries: reading it takes longer than most waits do.
-__device__ __forceinline__ bool opWaitSpin(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
+__device__ __forceinline__ bool opWaitSpin(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code, uint64_t limitNs = 2000000000ull) {
   uint64_t t0 = 0;
   for(uint32_t spins = 1;; spins++) {
     if(mbarTryWait(bar, parity)) return true;
@@ -123,7 +123,7 @@ __device__ __forceinline__ bool opWaitSpin(uint32_t bar, uint32_t parity, volati
       if(*abortFlag) return false;
       const uint64_t now = globalTimerNs();
       if(t0 == 0) t0 = now;
-      else if(now - t0 > 2000000000ull) {
+      else if(now - t0 > limitNs) {
         *abortFlag = 1;
         *status = code;
         __threadfence_system();
@@ -137,6 +137,14 @@ static __device__ __noinline__ bool opWaitOn(uint32_t bar, uint32_t parity, vola
 }
 __device__ __forceinline__ bool opWait(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {
   return mbarTryWait(bar, parity) != 0u || opWaitOn(bar, parity, abortFlag, status, code);
+}
+// For the sums of `slices` slices of K, which may take longer than any other wait: 20 us for each on top (the slowest, of rows on odd
+// boundaries, take 3).
+static __device__ __noinline__ bool opWaitSumsOn(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code, int slices) {
+  return opWaitSpin(bar, parity, abortFlag, status, code, 2000000000ull + 20000ull * (uint64_t)slices);
+}
+__device__ __forceinline__ bool opWaitSums(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code, int slices) {
+  return mbarTryWait(bar, parity) != 0u || opWaitSumsOn(bar, parity, abortFlag, status, code, slices);
 }
 // The same in line, for kernels that move registers between warpgroups (ptxas finds no allocation with a call in them).
 __device__ __forceinline__ bool opWaitInline(uint32_t bar, uint32_t parity, volatile int* abortFlag, volatile int* status, int code) {

@@ -126,6 +126,27 @@ def test_matmul_writes_its_columns_only(dtype, m, k, n):
         assert_within(multiply(dtype, x, w, None, 0, r, y), want, bound, residual)
         assert (whole[:, n:] == 7.0).all(), residual
 
+def test_matmul_of_the_longest_sums():
+    """Rows on odd boundaries, of the most channels that there may be: the sums take more than two seconds, which is no reason to give them up.
+    All but a few products are zeros, so the result is exact."""
+    m, k = 17, (1 << 30) - 1
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 2 * (m + 1) * k + (4 << 30):
+        pytest.skip("not enough memory")
+    x, w = torch.zeros(m, k, dtype=torch.float16, device="cuda"), torch.zeros(1, k, dtype=torch.float16, device="cuda")
+    places = [0, k // 2, k - 1]
+    for i, at in enumerate(places):
+        x[:, at] = torch.arange(m, device="cuda") % 7 + i
+        w[:, at] = 2 ** i
+    want = x[:, places].double() @ w[:, places].double().t()
+    y = multiply("fp16", x, w)
+    torch.cuda.synchronize()
+    assert torch.equal(y.double(), want)
+    one = torch.ones(32, 32, dtype=torch.float16, device="cuda")
+    assert (multiply("fp16", one, one) == 32).all()  # and no later call has anything to report
+    del x, w
+    torch.cuda.empty_cache()
+
 
 # ---- rope ----
 
