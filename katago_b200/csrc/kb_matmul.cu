@@ -5,7 +5,7 @@
 //                    of four bytes (rows may lie anywhere), which transpose them: a thread reads its rows and columns of a channel in
 //                    vectors and multiplies with the packed fp32 instructions, two columns at a time.  Where tiles are few, the
 //                    blocks of a cluster share K and add their sums in its order through distributed shared memory.
-//                    FMA-bound: 4096^3 50 TFLOP/s, two thirds of the units' cycles; shared memory is busy for another two thirds
+//                    FMA-bound: 4096^3 50 TFLOP/s, two thirds of the units' cycles; shared memory is busy for half of the time
 //                    (16 bytes per lane take three passes of it whatever lanes they repeat for).
 // matmulFewKernel    up to eight rows (fp32: 16): memory-bound, the weights are read once.  A block has four weight rows and cuts K
 //                    over its warps, whose sums are added in warp order.
