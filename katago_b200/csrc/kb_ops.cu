@@ -138,8 +138,15 @@ bool encodeTiled(
   cuuint64_t d[4], s[3];
   cuuint32_t b[4], one[4] = {1, 1, 1, 1};
   for(int i = 0; i < rank; i++) { d[i] = dims[i]; b[i] = box[i]; if(i > 0) s[i - 1] = strides[i - 1]; }
-  return fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto encode = [&]() {
+    return fn(map, type, (cuuint32_t)rank, const_cast<void*>(base), d, s, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  // a thread that has called nothing of the runtime that needs its device has no context yet, which this call, of the driver, does not see to
+  int dev = 0;
+  if(r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  return r == CUDA_SUCCESS;
 }
 
 void opMatmul(const MatmulArgs& given, void* stream) {

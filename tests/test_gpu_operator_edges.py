@@ -2,6 +2,7 @@
 calls that share memory or a graph in unusual ways.  (Bounds: operator_cases.py.)"""
 import ctypes
 import math
+import threading
 from fractions import Fraction
 
 import pytest
@@ -361,6 +362,52 @@ def test_attention_of_tiny_and_huge_scales(dtype, n, h, hk, d, scale):
         q, k = q * 1e-15, k * 1e-15
         want, bound = attention_reference(dtype, q, k, v, scale)
     assert_within(attend(dtype, q, k, v, empty_out(q, v), scale), want, bound)
+
+
+# ---- threads ----
+
+@pytest.mark.parametrize("op", ("matmul wide", "matmul few", "matmul skinny", "attention few", "attention", "attention fp32", "rope"))
+def test_the_first_call_of_a_thread(op):
+    """A thread that has not touched its device yet, with buffers that another one has made."""
+    g = seeded(op)
+    x, w = normal(g, 3000, 512, dtype="bf16"), normal(g, 256, 512, dtype="bf16", scale=0.05)
+    rows = {"matmul wide": 3000, "matmul few": 3, "matmul skinny": 100}.get(op, 0)
+    dtype = "fp32" if "fp32" in op else "fp16"
+    q, kv = normal(g, 2, 3 if op == "attention few" else 40, 4, 64, dtype=dtype), normal(g, 2, 300, 4, 64, dtype=dtype)
+    positions, freqs = torch.arange(80, device="cuda", dtype=torch.int32).view(2, 40, 1), torch.full((1, 32, 1), 0.1, device="cuda")
+    y, out = torch.zeros(max(rows, 1), 256, dtype=torch.bfloat16, device="cuda"), torch.zeros_like(q)
+    space = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+
+    def call():
+        if rows:
+            capi.matmul(PRECISION["bf16"], rows, 256, 512, x.data_ptr(), 512, w.data_ptr(), 512, y.data_ptr(), 256)
+        elif op == "rope":
+            capi.rope(PRECISION[dtype], 2, 40, 64, 64, positions.data_ptr(), 40, 1, freqs.data_ptr(), 1, 0, view(q), view(out), 4)
+        else:
+            b, n, h, d = q.shape
+            capi.cross_attention(PRECISION[dtype], b, n, 300, h, h, d, d, 0.125, view(q), view(kv), view(kv), view(out), workspace=space.data_ptr(),
+                                 workspace_bytes=1 << 22)
+
+    got = y if rows else out
+    call()
+    torch.cuda.synchronize()
+    want = got.clone()
+    got.zero_()
+    torch.cuda.synchronize()
+    errors = []
+
+    def work():
+        try:
+            call()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    t = threading.Thread(target=work)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert want.abs().sum() > 0 and torch.equal(got, want)
 
 
 # ---- graphs ----
