@@ -193,7 +193,8 @@ const char* kb_conv_noalloc_last_error(void);
  *     other way are refused, since that cannot be told from an overlap;
  *   - any alignment of the element type is taken; rows that start on 16-byte boundaries are fastest;
  *   - the kernels are enqueued on `stream` (a cudaStream_t of the current device, NULL = its default stream) and the call
- *     returns without waiting.  Calls may be captured into a graph, and made from several threads at once on different buffers;
+ *     returns without waiting.  Calls may be captured into a graph (on memory that exists by then: what cudaMallocAsync gives within
+ *     the capture is not device memory yet, and is refused), and made from several threads at once on different buffers;
  *   - nothing is allocated and nothing kept from one call to the next (but a status word for the library, at the first call);
  *   - non-zero and kb_last_error() as everywhere; a refused call has launched nothing.  A device-side wait that ran out (it never
  *     does in sound operation) is reported by the next call of an operator.
