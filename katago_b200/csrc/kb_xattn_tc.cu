@@ -14,8 +14,8 @@
 // p = 2^(scale log2(e) (s - ref)), where ref follows the row's maximum of s only when that has grown by more than 8 in the exponent (fp16: 4;
 // sums and O in fp32 lose nothing): only then is O rescaled, which costs a round trip of O through registers and a wait
 // for the product before.  The factor cancels in O / sum.  One multiply-add makes an exponent, from scale log2(e) ref rounded once.
-// Where that is above 512 its rounding would show (at 10^9 it is a hundred steps of the exponent): such a warp goes on
-// with a loop that subtracts ref from the scores first.
+// That rounding is half an fp32 step of such a score: at 4096 2^-12 of the exponent, at 10^9 64 of it.  So a warp with a reference
+// above 4096 goes on with a loop that subtracts ref from the scores first (2 x 4096 x 8192 tokens: 1.23 ms, 0.51 with any smaller).
 //
 // Keys that are not attended (masked, or behind the last one) may hold anything.  In shared memory their rows of V are cleared and
 // their rows of K are replaced by that of an attended key of the tile: so their scores are scores of the row that lie no higher
@@ -52,7 +52,7 @@ constexpr int XT_HALF = 128 * 64 * 2;  // bytes of 128 rows x 64 channels
 // are 2^-25 of the reference's still have all their bits.  (bf16 has the range of fp32.)
 template <typename T> constexpr float XT_UP = std::is_same<T, __half>::value ? 11.0f : 0.0f;
 template <typename T> constexpr float XT_GROW = std::is_same<T, __half>::value ? 4.0f : 8.0f;  // of the exponent, before the reference follows
-constexpr float XT_FAR = 512.0f;
+constexpr float XT_FAR = 4096.0f;
 enum { XT_ALL, XT_SOME, XT_NONE };
 constexpr int XT_SORT = 128;  // sequences that a block ranks
 
